@@ -298,6 +298,64 @@ def bind(native):
         def free(self):
             native.kvCacheFree(self.cacheId)
 
+    def qkNormRope(q, k, gammaQ, gammaK, positions=None, offset=0, rotaryDims=None, interleaved=False, theta=10000.0, eps=1e-6):
+        """Queries [B, Hq, S, D] and keys [B, Hk, S, D], each head normed (gains [D]) and rotated by its position; see
+        mni_qk_norm_rope.  positions: an int buffer's id (native.createDataset), or None for 0 .. S - 1."""
+        ids = native.qkNormRope(q._id, k._id, gammaQ._id, gammaK._id, positions, offset, q.shape[-1] if rotaryDims is None else rotaryDims,
+                                interleaved, theta, eps)
+        return Tensor(ids[0], q.shape), Tensor(ids[1], k.shape)
+
+    class PagedKvCache:
+        """Keys and values of many sequences in one pool of pages; see mni_paged_cache_create.  Sequences are ids from add()
+        or fork(); the calls that take several take a list of them."""
+
+        def __init__(self, maxSequences, maxSeqLen, numPages, pageSize, numKvHeads, headDim, quantized=True, tracked=False):
+            self.cacheId = native.pagedCacheCreate(maxSequences, maxSeqLen, numPages, pageSize, numKvHeads, headDim, quantized, tracked)
+
+        def add(self):
+            return native.pagedCacheAdd(self.cacheId)
+
+        def fork(self, seq):
+            return native.pagedCacheFork(self.cacheId, seq)
+
+        def drop(self, seq):
+            native.pagedCacheDrop(self.cacheId, seq)
+
+        def length(self, seq):
+            return native.pagedCacheLen(self.cacheId, seq)
+
+        def seen(self, seq):
+            return native.pagedCacheSeen(self.cacheId, seq)
+
+        def freePages(self):
+            return native.pagedCacheFreePages(self.cacheId)
+
+        def append(self, seqs, k, v, counts=None):
+            native.pagedCacheAppend(self.cacheId, seqs, k._id, v._id, counts)
+
+        def truncate(self, seqs, lens):
+            native.pagedCacheTruncate(self.cacheId, seqs, lens)
+
+        def attend(self, seqs, q, scale, accumulate=False):
+            return Tensor(native.pagedCacheAttend(self.cacheId, seqs, q._id, scale, accumulate))
+
+        def addWeights(self, seqs, w):
+            native.pagedCacheAddWeights(self.cacheId, seqs, w._id)
+
+        def evict(self, seqs, budget, recent=0):
+            native.pagedCacheEvict(self.cacheId, seqs, budget, recent)
+
+        def track(self, seqs):
+            """(weights, positions): a tensor [n, heads, longest] and the id of an int buffer of as many values."""
+            w, p = native.pagedCacheTrack(self.cacheId, seqs)
+            return Tensor(w), p
+
+        def read(self, seq):
+            return tuple(Tensor(i) for i in native.pagedCacheRead(self.cacheId, seq))
+
+        def free(self):
+            native.pagedCacheFree(self.cacheId)
+
     class Adam:  # src/optimizer.ts:33-70: options object, defaults lr 6e-4, beta2 0.95
         def __init__(self, parameters, lr=6e-4, beta1=0.9, beta2=0.95, eps=1e-8, weightDecay=0.0):
             self.parameters = list(parameters)
@@ -340,4 +398,4 @@ def bind(native):
     return SimpleNamespace(native=native, Embedding=Embedding, crossEntropyLossGpu=crossEntropyLossGpu, dropout=dropout,
                            residualLayerNorm=residualLayerNorm, tile=tile, GradScaler=GradScaler, Tensor=Tensor, Parameter=Parameter, Module=Module, Linear=Linear, ReLU=ReLU,
                            GELU=GELU, mseLoss=mseLoss, crossEntropyLoss=crossEntropyLoss, softmax=softmax, biasGelu=biasGelu, layerNorm=layerNorm,
-                           flashAttention=flashAttention, KvCache=KvCache, Adam=Adam)
+                           flashAttention=flashAttention, KvCache=KvCache, qkNormRope=qkNormRope, PagedKvCache=PagedKvCache, Adam=Adam)

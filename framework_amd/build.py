@@ -15,8 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "lib", "obj")
 LIB = os.path.join(HERE, "lib", "libmni_rocm.so")
-SOURCES = ["device.hip", "gemm_mfma.hip", "gemm_direct.hip", "gemm_panel.hip", "gemm_tiny.hip", "gemm_fewrows.hip", "gemm_outer.hip", "gemm_skinny.hip", "gemm_gemv.hip", "gemm_fewrows_nt.hip", "gemm.hip", "elementwise.hip", "yardstick.hip", "attention.hip", "sequence.hip", "engine.hip"]
-HEADERS = ["common.h", "gemm_internal.h", os.path.join("..", "..", "include", "mni_rocm.h")]
+SOURCES = ["device.hip", "gemm_mfma.hip", "gemm_direct.hip", "gemm_panel.hip", "gemm_tiny.hip", "gemm_fewrows.hip", "gemm_outer.hip", "gemm_skinny.hip", "gemm_gemv.hip", "gemm_fewrows_nt.hip", "gemm.hip", "elementwise.hip", "yardstick.hip", "attention.hip", "rotary.hip", "paged_cache.hip", "sequence.hip", "engine.hip"]
+HEADERS = ["common.h", "gemm_internal.h", "lanes.h", "paged_cache.h", os.path.join("..", "..", "include", "mni_rocm.h")]
 
 # -packed-fp32-ops is switched off for device code: hipcc must not form
 # v_pk_*_f32 from ordinary float arithmetic on this target.
@@ -103,7 +103,7 @@ def build_node_addon(force=False, verbose=True):
         if verbose:
             print("node_api.h not found: Node addon not built")
         return None
-    if force or _stale(NODE_ADDON, [src, LIB, os.path.normpath(os.path.join(CSRC, HEADERS[2]))]):
+    if force or _stale(NODE_ADDON, [src, LIB, os.path.normpath(os.path.join(CSRC, HEADERS[-1]))]):
         _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-I" + NODE_INCLUDE, src, "-o", NODE_ADDON,
               "-L" + os.path.dirname(LIB), "-lmni_rocm", "-Wl,-rpath,$ORIGIN"])
         if verbose:

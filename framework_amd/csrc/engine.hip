@@ -19,6 +19,7 @@
 
 #include "common.h"
 #include "gemm_internal.h"
+#include "paged_cache.h"
 #include <functional>
 
 namespace mni {
@@ -64,7 +65,7 @@ enum Op {  // subset of src/native/src/autograd.rs:28-62 plus the fused Linear
     OP_SUM, OP_MEAN, OP_VIEW, OP_PERMUTE, OP_CONTIGUOUS, OP_CROSSENTROPY, OP_LINEAR,
     OP_SOFTMAX, OP_FLASHATTENTION, OP_BIASGELU,
     OP_EXP, OP_LOG, OP_DIV, OP_SIGMOID, OP_POW, OP_MAX, OP_LAYERNORM,
-    OP_EMBEDDING, OP_DROPOUT, OP_RESIDUALLAYERNORM, OP_MSEROWS
+    OP_EMBEDDING, OP_DROPOUT, OP_RESIDUALLAYERNORM, OP_MSEROWS, OP_NORMROPE
 };
 
 // src/native/src/autograd.rs:65-70 TapeEntry
@@ -85,6 +86,7 @@ struct Entry {
     BufP mse_grad_for_ones;         // fused mseLoss: d loss / d prediction for an upstream gradient of ones, computed with the loss
     int64_t ce_n = 0, ce_v = 0;
     uint64_t rng_seed = 0, rng_offset = 0;  // dropout: where its mask starts in the random stream
+    mni_rope_desc rope = {};                // norm + rotation: its plan (no operands); `targets` holds the positions
 };
 
 struct Tape {
@@ -99,6 +101,21 @@ struct KvCache {
     bool quantized = false;
     std::shared_ptr<void> keys, vals;      // [bh, max_seq, d] float or int8
     std::shared_ptr<void> kscale, vscale;  // [bh, max_seq] float (quantized only)
+};
+
+// A sequence of a paged cache: what the host knows of it.  `floor`: rows left by its last eviction, which truncation
+// does not go below.
+struct PagedSequence {
+    bool live = false;
+    int64_t len = 0, seen = 0, floor = 0;
+    std::vector<int32_t> pages;
+};
+struct PagedCache {
+    PagedPool pool = {};
+    std::vector<std::shared_ptr<void>> blocks;  // the pool's device memory
+    std::vector<int32_t> free_pages, holders;   // pages nobody holds (the next one last); sequences that hold each page
+    std::vector<PagedSequence> seqs;
+    std::vector<uint32_t> free_seqs;
 };
 
 // ops/data.rs:13-27 IntBuffer, on the device.  lo / hi bound the values it can
@@ -117,6 +134,8 @@ struct Engine {
     Tape tape;
     std::map<uint32_t, KvCache> kv_caches;  // lib.rs:23-24
     uint32_t next_kv_cache_id = 1;          // lib.rs:36
+    std::map<uint32_t, PagedCache> paged_caches;
+    uint32_t next_paged_cache_id = 1;
     std::vector<IntBuf> int_bufs;           // ops/data.rs:24-27 IntStore
     std::vector<uint32_t> int_free;
     // Random numbers: Philox blocks (seed, offset) on the device, a Mersenne
@@ -1811,6 +1830,455 @@ static int residual_layernorm_backward(uint32_t grad, const Entry &e, int64_t *o
     return MNI_OK;
 }
 
+// ---- norm and rotation of queries and keys (rotary.hip) -----------------------------------------------
+// Where a [B, H, S, D] tensor's rows lie; gathered first if its last extent is not contiguous.
+static bool rope_rows(const Tensor &t, mni_rope_heads *o, BufP *keep) {
+    Shape strides = t.strides;
+    *keep = t.buf;
+    if (strides[3] != 1 && t.shape[3] != 1) {
+        *keep = contiguous_buf(t);
+        if (!*keep) return false;
+        strides = compute_strides(t.shape);
+    }
+    o->x = (*keep)->p;
+    o->heads = t.shape[1];
+    o->batch_stride = strides[0]; o->head_stride = strides[1]; o->token_stride = strides[2];
+    return true;
+}
+static int norm_rope_op(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k, uint32_t positions, int64_t offset, int64_t rotary_dims,
+                        int interleaved, double theta, double eps, uint32_t *out_ids) {
+    Tensor *Q = get(q), *K = get(k), *Gq = get(gamma_q), *Gk = get(gamma_k);
+    if (!Q || !K || !Gq || !Gk) return MNI_ERR_FREED;
+    if (Q->shape.size() != 4 || K->shape.size() != 4) return set_error(MNI_ERR_INVALID, "qk_norm_rope: q and k must be [B, H, S, D]");
+    const Shape qs = Q->shape, ks = K->shape;
+    if (qs[0] != ks[0] || qs[2] != ks[2] || qs[3] != ks[3]) return set_error(MNI_ERR_INVALID, "qk_norm_rope: q and k differ in batch, length or head_dim");
+    const int64_t d = qs[3];
+    if (Gq->shape != Shape{d} || Gk->shape != Shape{d}) return set_error(MNI_ERR_INVALID, "qk_norm_rope: the gains must be [%lld]", (long long)d);
+    mni_rope_desc r = {};
+    r.batch = qs[0]; r.seq = qs[2]; r.head_dim = d; r.rotary_dims = rotary_dims;
+    r.offset = offset; r.theta = theta; r.eps = eps; r.interleaved = interleaved;
+    std::shared_ptr<void> at;
+    if (positions != MNI_BAD_ID) {
+        IntBuf *b = get_int(positions);
+        if (!b) return MNI_ERR_FREED;
+        if (b->len != r.seq && b->len != r.batch * r.seq)
+            return set_error(MNI_ERR_INVALID, "qk_norm_rope: positions hold %lld values, expected %lld or %lld", (long long)b->len, (long long)r.seq,
+                             (long long)(r.batch * r.seq));
+        at = b->data;
+        r.positions = (const int32_t *)at.get();
+        r.position_stride = b->len == r.seq ? 0 : r.seq;
+    }
+    Entry plan;
+    plan.op = OP_NORMROPE; plan.n_inputs = 2; plan.targets = at; plan.rope = r;
+    BufP keep_q, keep_k, gq = contiguous_buf(*Gq), gk = contiguous_buf(*Gk);
+    BufP oq = new_buf((size_t)shape_size(qs)), ok = oq ? new_buf((size_t)shape_size(ks)) : nullptr;
+    if (!ok || !gq || !gk || !rope_rows(*Q, &r.q, &keep_q) || !rope_rows(*K, &r.k, &keep_k)) return MNI_ERR_NOMEM;
+    r.q.gamma = gq->p; r.k.gamma = gk->p;
+    r.q.out = oq->p; r.k.out = ok->p;
+    MNI_TRY(mni_rocm_qk_norm_rope(&r));
+    out_ids[0] = insert_contig(std::move(oq), qs);
+    out_ids[1] = insert_contig(std::move(ok), ks);
+    Entry eq = plan, ek = plan;
+    eq.output_id = out_ids[0]; eq.inputs[0] = q; eq.inputs[1] = gamma_q;
+    ek.output_id = out_ids[1]; ek.inputs[0] = k; ek.inputs[1] = gamma_k;
+    eng().tape.record(std::move(eq));
+    eng().tape.record(std::move(ek));
+    return MNI_OK;
+}
+static int norm_rope_backward(uint32_t grad, const Entry &e, int64_t *out) {
+    Tensor *X = get(e.inputs[0]), *Gm = get(e.inputs[1]), *G = get(grad);
+    if (!X || !Gm || !G) return MNI_ERR_FREED;
+    const Shape shape = X->shape, gshape = Gm->shape;
+    mni_rope_desc r = e.rope;
+    BufP keep, gm = contiguous_buf(*Gm), g = contiguous_buf(*G);
+    BufP dx = (gm && g) ? new_buf((size_t)X->size) : nullptr, dgamma = dx ? new_buf((size_t)Gm->size) : nullptr;
+    if (!dgamma || !rope_rows(*X, &r.q, &keep)) return MNI_ERR_NOMEM;
+    r.q.gamma = gm->p; r.q.grad = g->p; r.q.dx = dx->p; r.q.dgamma = dgamma->p;
+    MNI_TRY(mni_rocm_qk_norm_rope_backward(&r));
+    out[0] = insert_contig(std::move(dx), shape);
+    out[1] = insert_contig(std::move(dgamma), gshape);
+    return MNI_OK;
+}
+
+// ---- paged KV cache (paged_cache.hip) ---------------------------------------------------------------------
+// The host decides which page goes where, from lengths that it knows without asking the device; kernels get the
+// sequences of a call in their arguments, so a decoding step uploads nothing and waits for nothing.
+static PagedCache *paged(uint32_t id) {
+    auto it = eng().paged_caches.find(id);
+    if (it != eng().paged_caches.end()) return &it->second;
+    set_error(MNI_ERR_INVALID, "invalid paged cache id: %u", id);
+    return nullptr;
+}
+static PagedSequence *paged_seq(PagedCache &c, uint32_t seq) {
+    if (seq < c.seqs.size() && c.seqs[seq].live) return &c.seqs[seq];
+    set_error(MNI_ERR_INVALID, "invalid paged cache sequence id: %u", seq);
+    return nullptr;
+}
+// Every id names a sequence; none twice where `distinct`.
+static int paged_check(PagedCache &c, const uint32_t *seqs, size_t n, bool distinct, const char *what) {
+    if (n && !seqs) return set_error(MNI_ERR_INVALID, "paged cache %s: null sequence list", what);
+    std::vector<char> used(distinct ? c.seqs.size() : 0, 0);
+    for (size_t i = 0; i < n; ++i) {
+        if (!paged_seq(c, seqs[i])) return MNI_ERR_INVALID;
+        if (!distinct) continue;
+        if (used[seqs[i]]) return set_error(MNI_ERR_INVALID, "paged cache %s: sequence %u occurs twice", what, seqs[i]);
+        used[seqs[i]] = 1;
+    }
+    return MNI_OK;
+}
+static int64_t paged_pages(const PagedCache &c, int64_t tokens) { return (tokens + c.pool.page - 1) >> c.pool.shift; }
+static int32_t paged_take(PagedCache &c) {
+    const int32_t page = c.free_pages.back();
+    c.free_pages.pop_back();
+    c.holders[page] = 1;
+    return page;
+}
+static void paged_release(PagedCache &c, PagedSequence &s, int64_t keep) {  // the last pages first: the next sequence takes them in order
+    while ((int64_t)s.pages.size() > keep) {
+        const int32_t page = s.pages.back();
+        s.pages.pop_back();
+        if (--c.holders[page] == 0) c.free_pages.push_back(page);
+    }
+}
+static int64_t paged_entry(const PagedCache &c, uint32_t seq, int64_t page) { return (int64_t)seq * c.pool.max_pages + page; }
+// Own copies of the pages [from, to) of a sequence that others hold too.  The caller has made sure of enough pages.
+static int paged_unshare(PagedCache &c, uint32_t seq, int64_t from, int64_t to, PagedCopies &copies) {
+    PagedSequence &s = c.seqs[seq];
+    for (int64_t j = from; j < to; ++j) {
+        const int32_t page = s.pages[j];
+        if (c.holders[page] <= 1) continue;
+        if (copies.n == PAGED_PAIRS / 2) {
+            MNI_TRY(k_paged_copy(c.pool, copies));
+            copies.n = 0;
+        }
+        copies.at[copies.n] = paged_entry(c, seq, j);
+        copies.from[copies.n] = page;
+        --c.holders[page];
+        s.pages[j] = copies.to[copies.n++] = paged_take(c);
+    }
+    return MNI_OK;
+}
+static PagedSeqs paged_batch(const PagedCache &c, const uint32_t *seqs, size_t first, size_t n) {
+    PagedSeqs s = {};
+    s.n = (int)std::min<size_t>(PAGED_BATCH, n - first);
+    for (int i = 0; i < s.n; ++i) {
+        s.slot[i] = (int32_t)seqs[first + i];
+        s.len[i] = (int32_t)c.seqs[seqs[first + i]].len;
+    }
+    return s;
+}
+static int64_t paged_longest(const PagedCache &c, const uint32_t *seqs, size_t n) {
+    int64_t longest = 0;
+    for (size_t i = 0; i < n; ++i) longest = std::max(longest, c.seqs[seqs[i]].len);
+    return longest;
+}
+
+static uint32_t paged_create(int64_t max_sequences, int64_t max_seq_len, int64_t num_pages, int64_t page_size, int64_t heads, int64_t d, bool quantized,
+                             bool tracked) {
+    const int64_t most = (int64_t)1 << 30;
+    if (max_sequences < 1 || max_seq_len < 1 || num_pages < 1 || max_sequences > (1 << 20) || max_seq_len > most || num_pages > most) {
+        set_error(MNI_ERR_INVALID, "paged cache: sequences, their length and the pages must be from 1 up to 2^20, 2^30 and 2^30");
+        return MNI_BAD_ID;
+    }
+    if (page_size < 1 || page_size > 1024 || (page_size & (page_size - 1))) {
+        set_error(MNI_ERR_INVALID, "paged cache: page_size %lld is no power of two up to 1024", (long long)page_size);
+        return MNI_BAD_ID;
+    }
+    if (heads < 1 || heads > 256 || d < 1 || d > 256) {
+        set_error(MNI_ERR_INVALID, "paged cache: kv_heads and head_dim must be from 1 to 256, got %lld and %lld", (long long)heads, (long long)d);
+        return MNI_BAD_ID;
+    }
+    PagedCache c;
+    PagedPool &p = c.pool;
+    p.heads = (int)heads; p.d = (int)d; p.page = (int)page_size; p.quantized = quantized ? 1 : 0;
+    while ((1 << p.shift) < p.page) ++p.shift;
+    p.max_len = max_seq_len;
+    p.max_pages = paged_pages(c, max_seq_len);
+    // in doubles first: a size no card has must not wrap around
+    const double rows_d = (double)num_pages * heads * page_size, track_d = tracked ? (double)max_sequences * heads * max_seq_len : 0.0;
+    if (rows_d * d * (quantized ? 1 : 4) > 1e14 || track_d > 1e14 || (double)max_sequences * p.max_pages > 1e14) {
+        set_error(MNI_ERR_NOMEM, "paged cache: a pool of that size does not fit any device");
+        return MNI_BAD_ID;
+    }
+    const size_t rows = (size_t)(num_pages * heads * page_size), track = (size_t)(max_sequences * heads * max_seq_len);
+    auto block = [&](size_t bytes) {
+        std::shared_ptr<void> b = dev_block(bytes);
+        if (b) c.blocks.push_back(b);
+        return b.get();
+    };
+    if (!(p.k = block(rows * d * (quantized ? 1 : 4))) || !(p.v = block(rows * d * (quantized ? 1 : 4)))) return MNI_BAD_ID;
+    if (quantized && (!(p.kscale = (float *)block(rows * 4)) || !(p.vscale = (float *)block(rows * 4)))) return MNI_BAD_ID;
+    if (!(p.table = (int32_t *)block((size_t)(max_sequences * p.max_pages) * 4))) return MNI_BAD_ID;
+    if (tracked && (!(p.weight = (float *)block(track * 4)) || !(p.pos = (int32_t *)block(track * 4)))) return MNI_BAD_ID;
+    c.holders.assign((size_t)num_pages, 0);
+    c.free_pages.reserve((size_t)num_pages);
+    for (int64_t i = num_pages; i-- > 0;) c.free_pages.push_back((int32_t)i);
+    c.seqs.resize((size_t)max_sequences);
+    c.free_seqs.reserve((size_t)max_sequences);
+    for (int64_t i = max_sequences; i-- > 0;) c.free_seqs.push_back((uint32_t)i);
+    Engine &e = eng();
+    const uint32_t id = e.next_paged_cache_id++;
+    e.paged_caches[id] = std::move(c);
+    return id;
+}
+static uint32_t paged_add(PagedCache &c) {
+    if (c.free_seqs.empty()) { set_error(MNI_ERR_INVALID, "paged cache: all %zu sequences are in use", c.seqs.size()); return MNI_BAD_ID; }
+    const uint32_t seq = c.free_seqs.back();
+    c.free_seqs.pop_back();
+    c.seqs[seq] = PagedSequence();
+    c.seqs[seq].live = true;
+    return seq;
+}
+static uint32_t paged_fork(PagedCache &c, uint32_t from) {
+    if (!paged_seq(c, from)) return MNI_BAD_ID;
+    const uint32_t seq = paged_add(c);
+    if (seq == MNI_BAD_ID) return MNI_BAD_ID;
+    if (k_paged_fork(c.pool, (int32_t)from, (int32_t)seq, c.seqs[from].len) != MNI_OK) {
+        c.seqs[seq] = PagedSequence();
+        c.free_seqs.push_back(seq);
+        return MNI_BAD_ID;
+    }
+    c.seqs[seq] = c.seqs[from];
+    for (int32_t page : c.seqs[seq].pages) ++c.holders[page];
+    return seq;
+}
+// New table entries: up to a few hundred travel in a launch's arguments, more go up as the runs that they are.
+static int paged_write_table(PagedCache &c, const uint32_t *seqs, const std::vector<int64_t> &had, size_t total) {
+    if (total == 0) return MNI_OK;
+    if (total > 4 * PAGED_PAIRS / 2) {
+        for (size_t i = 0; i < had.size(); ++i) {
+            const std::vector<int32_t> &pages = c.seqs[seqs[i]].pages;
+            for (size_t j = (size_t)had[i]; j < pages.size(); j += DeviceCtx::STAGE_BYTES / 4)
+                MNI_TRY(upload_small(c.pool.table + paged_entry(c, seqs[i], (int64_t)j), pages.data() + j,
+                                     std::min<size_t>(DeviceCtx::STAGE_BYTES / 4, pages.size() - j) * 4));
+        }
+        return MNI_OK;
+    }
+    PagedTableWrite w;
+    w.n = 0;
+    for (size_t i = 0; i < had.size(); ++i) {
+        const std::vector<int32_t> &pages = c.seqs[seqs[i]].pages;
+        for (size_t j = (size_t)had[i]; j < pages.size(); ++j) {
+            w.at[w.n] = paged_entry(c, seqs[i], (int64_t)j);
+            w.page[w.n++] = pages[j];
+            if (w.n == PAGED_PAIRS / 2) {
+                MNI_TRY(k_paged_table(c.pool, w));
+                w.n = 0;
+            }
+        }
+    }
+    return k_paged_table(c.pool, w);
+}
+static int paged_append(PagedCache &c, const uint32_t *seqs, size_t n, uint32_t k, uint32_t v, const int64_t *counts) {
+    MNI_TRY(paged_check(c, seqs, n, true, "append"));
+    Tensor *K = get(k), *V = get(v);
+    if (!K || !V) return MNI_ERR_FREED;
+    const PagedPool &p = c.pool;
+    if (K->shape != V->shape) return set_error(MNI_ERR_INVALID, "paged cache append: k/v shapes must match");
+    if (K->shape.size() != 4 || K->shape[0] != (int64_t)n || K->shape[1] != p.heads || K->shape[3] != p.d)
+        return set_error(MNI_ERR_INVALID, "paged cache append: expected [%zu, %d, T, %d], got %s", n, p.heads, p.d, shape_text(K->shape).c_str());
+    const int64_t tokens = K->shape[2];
+    if (tokens > ((int64_t)1 << 31) / (PAGED_BATCH * (int64_t)p.heads))
+        return set_error(MNI_ERR_INVALID, "paged cache append: %lld tokens of %d heads are too many for one call", (long long)tokens, p.heads);
+    // everything is checked before anything changes
+    int64_t need = 0;
+    std::map<int32_t, int> left;  // shared last pages: holders that still share them
+    for (size_t i = 0; i < n; ++i) {
+        const PagedSequence &s = c.seqs[seqs[i]];
+        const int64_t count = counts ? counts[i] : tokens;
+        if (count < 0 || count > tokens) return set_error(MNI_ERR_INVALID, "paged cache append: counts[%zu] = %lld of %lld tokens", i, (long long)count, (long long)tokens);
+        if (s.len + count > p.max_len || s.seen + count > INT32_MAX)
+            return set_error(MNI_ERR_INVALID, "paged cache append: sequence %u is full (len=%lld, max_seq_len=%lld)", seqs[i], (long long)s.len, (long long)p.max_len);
+        need += paged_pages(c, s.len + count) - (int64_t)s.pages.size();
+        if (count > 0 && (s.len & (p.page - 1))) {
+            const int32_t last = s.pages.back();
+            if (c.holders[last] > 1) {
+                auto it = left.emplace(last, c.holders[last]).first;
+                if (it->second > 1) { ++need; --it->second; }
+            }
+        }
+    }
+    if (need > (int64_t)c.free_pages.size())
+        return set_error(MNI_ERR_INVALID, "paged cache append: the cache is full (%lld pages wanted, %zu free)", (long long)need, c.free_pages.size());
+    if (n == 0 || tokens == 0) return MNI_OK;
+    auto rows = [&](const Tensor &t, BufP *keep, Shape *strides) {
+        *strides = t.strides;
+        *keep = t.buf;
+        if ((*strides)[3] != 1 && p.d != 1) {
+            *keep = contiguous_buf(t);
+            *strides = compute_strides(t.shape);
+        }
+        return *keep != nullptr;
+    };
+    BufP kb, vb;
+    Shape kst, vst;
+    if (!rows(*K, &kb, &kst) || !rows(*V, &vb, &vst)) return MNI_ERR_NOMEM;
+    PagedNew in;
+    in.k_seq = kst[0]; in.k_head = kst[1]; in.k_token = kst[2];
+    in.v_seq = vst[0]; in.v_head = vst[1]; in.v_token = vst[2];
+    in.tokens = (int)tokens;
+    PagedCopies copies;
+    copies.n = 0;
+    std::vector<int64_t> had(n);
+    size_t total = 0;
+    for (size_t i = 0; i < n; ++i) {
+        PagedSequence &s = c.seqs[seqs[i]];
+        const int64_t count = counts ? counts[i] : tokens;
+        if (count > 0 && (s.len & (p.page - 1))) MNI_TRY(paged_unshare(c, seqs[i], (int64_t)s.pages.size() - 1, (int64_t)s.pages.size(), copies));
+        had[i] = (int64_t)s.pages.size();
+        while ((int64_t)s.pages.size() < paged_pages(c, s.len + count)) { s.pages.push_back(paged_take(c)); ++total; }
+    }
+    MNI_TRY(k_paged_copy(p, copies));
+    if (tokens > 1) MNI_TRY(paged_write_table(c, seqs, had, total));
+    for (size_t first = 0; first < n; first += PAGED_BATCH) {
+        PagedAppend a;
+        a.n = (int)std::min<size_t>(PAGED_BATCH, n - first);
+        for (int i = 0; i < a.n; ++i) {
+            PagedSequence &s = c.seqs[seqs[first + i]];
+            a.slot[i] = (int32_t)seqs[first + i];
+            a.len[i] = (int32_t)s.len;
+            a.count[i] = (int32_t)(counts ? counts[first + i] : tokens);
+            a.seen[i] = (int32_t)s.seen;
+            a.page[i] = tokens == 1 && (int64_t)s.pages.size() > had[first + i] ? s.pages.back() : -1;
+            s.len += a.count[i];
+            s.seen += a.count[i];
+        }
+        in.k = kb->p + (int64_t)first * in.k_seq;
+        in.v = vb->p + (int64_t)first * in.v_seq;
+        MNI_TRY(k_paged_append(p, in, a));
+    }
+    return MNI_OK;
+}
+static int paged_truncate(PagedCache &c, const uint32_t *seqs, size_t n, const int64_t *lens) {
+    MNI_TRY(paged_check(c, seqs, n, true, "truncate"));
+    if (n && !lens) return set_error(MNI_ERR_INVALID, "paged cache truncate: null lengths");
+    for (size_t i = 0; i < n; ++i) {
+        const PagedSequence &s = c.seqs[seqs[i]];
+        if (lens[i] < s.floor || lens[i] > s.len)
+            return set_error(MNI_ERR_INVALID, "paged cache truncate: sequence %u of %lld rows%s cannot be cut to %lld", seqs[i], (long long)s.len,
+                             s.floor ? " (evicted)" : "", (long long)lens[i]);
+    }
+    for (size_t i = n; i-- > 0;) {
+        PagedSequence &s = c.seqs[seqs[i]];
+        s.seen -= s.len - lens[i];
+        s.len = lens[i];
+        paged_release(c, s, paged_pages(c, s.len));
+    }
+    return MNI_OK;
+}
+static uint32_t paged_attend(PagedCache &c, const uint32_t *seqs, size_t n, uint32_t q, float scale, bool accumulate) {
+    if (accumulate && !c.pool.weight) { set_error(MNI_ERR_INVALID, "paged cache attend: accumulate needs a tracked cache"); return MNI_BAD_ID; }
+    if (paged_check(c, seqs, n, accumulate, "attend") != MNI_OK) return MNI_BAD_ID;
+    Tensor *Q = get(q);
+    if (!Q) return MNI_BAD_ID;
+    const PagedPool &p = c.pool;
+    const Shape shape = Q->shape;
+    const int nd = (int)shape.size();
+    const int64_t heads = nd == 4 ? shape[1] : nd == 3 && n ? shape[0] / (int64_t)n : 0;
+    if ((nd != 4 && nd != 3) || shape[0] != (nd == 4 ? (int64_t)n : heads * (int64_t)n) || shape[nd - 2] != 1 || shape[nd - 1] != p.d) {
+        set_error(MNI_ERR_INVALID, "paged cache attend: expected [%zu, H, 1, %d] or [%zu * H, 1, %d], got %s", n, p.d, n, p.d, shape_text(shape).c_str());
+        return MNI_BAD_ID;
+    }
+    if (n && (heads < p.heads || heads % p.heads || heads > 4096)) {
+        set_error(MNI_ERR_INVALID, "paged cache attend: %lld query heads are no multiple of %d key heads (or beyond 4096)", (long long)heads, p.heads);
+        return MNI_BAD_ID;
+    }
+    BufP qb = contiguous_buf(*Q), out = qb ? new_buf((size_t)Q->size) : nullptr;
+    if (!out) return MNI_BAD_ID;
+    for (size_t first = 0; first < n; first += PAGED_BATCH) {
+        const int64_t at = (int64_t)first * heads * p.d;
+        if (k_paged_attend(p, paged_batch(c, seqs, first, n), qb->p + at, out->p + at, (int)heads, scale, accumulate) != MNI_OK) return MNI_BAD_ID;
+    }
+    return insert_contig(std::move(out), shape);
+}
+static int paged_add_weights(PagedCache &c, const uint32_t *seqs, size_t n, uint32_t w) {
+    const PagedPool &p = c.pool;
+    if (!p.weight) return set_error(MNI_ERR_INVALID, "paged cache add_weights: the cache is not tracked");
+    MNI_TRY(paged_check(c, seqs, n, true, "add_weights"));
+    Tensor *W = get(w);
+    if (!W) return MNI_ERR_FREED;
+    const int64_t longest = paged_longest(c, seqs, n);
+    if (W->shape.size() != 3 || W->shape[0] != (int64_t)n || W->shape[1] != p.heads || W->shape[2] < longest)
+        return set_error(MNI_ERR_INVALID, "paged cache add_weights: expected [%zu, %d, at least %lld], got %s", n, p.heads, (long long)longest, shape_text(W->shape).c_str());
+    const int64_t width = W->shape[2];
+    BufP wb = contiguous_buf(*W);
+    if (!wb) return MNI_ERR_NOMEM;
+    for (size_t first = 0; first < n; first += PAGED_BATCH)
+        MNI_TRY(k_paged_add_weights(p, paged_batch(c, seqs, first, n), wb->p + (int64_t)first * p.heads * width, width));
+    return MNI_OK;
+}
+static int paged_evict(PagedCache &c, const uint32_t *seqs, size_t n, int64_t budget, int64_t recent) {
+    const PagedPool &p = c.pool;
+    if (!p.weight) return set_error(MNI_ERR_INVALID, "paged cache evict: the cache is not tracked");
+    MNI_TRY(paged_check(c, seqs, n, true, "evict"));
+    if (budget < 0 || recent < 0 || recent > budget)
+        return set_error(MNI_ERR_INVALID, "paged cache evict: budget %lld must hold the %lld recent tokens", (long long)budget, (long long)recent);
+    const int64_t keep = paged_pages(c, std::min(budget, p.max_len));
+    int64_t need = 0;
+    std::map<int32_t, int> left;
+    for (size_t i = 0; i < n; ++i) {
+        const PagedSequence &s = c.seqs[seqs[i]];
+        if (s.len <= budget) continue;
+        for (int64_t j = 0; j < keep; ++j)
+            if (c.holders[s.pages[j]] > 1) {
+                auto it = left.emplace(s.pages[j], c.holders[s.pages[j]]).first;
+                if (it->second > 1) { ++need; --it->second; }
+            }
+    }
+    if (need > (int64_t)c.free_pages.size())
+        return set_error(MNI_ERR_INVALID, "paged cache evict: %lld pages are shared and only %zu are free for copies", (long long)need, c.free_pages.size());
+    PagedCopies copies;
+    copies.n = 0;
+    for (size_t i = 0; i < n; ++i)
+        if (c.seqs[seqs[i]].len > budget) MNI_TRY(paged_unshare(c, seqs[i], 0, keep, copies));
+    MNI_TRY(k_paged_copy(p, copies));
+    for (size_t first = 0; first < n; first += PAGED_BATCH) {
+        const PagedSeqs s = paged_batch(c, seqs, first, n);
+        int32_t seen[PAGED_BATCH];
+        for (int i = 0; i < s.n; ++i) seen[i] = (int32_t)c.seqs[seqs[first + i]].seen;
+        MNI_TRY(k_paged_evict(p, s, seen, (int)std::min<int64_t>(budget, INT32_MAX), (int)std::min<int64_t>(recent, INT32_MAX)));
+    }
+    for (size_t i = n; i-- > 0;) {
+        PagedSequence &s = c.seqs[seqs[i]];
+        if (s.len <= budget) continue;
+        s.len = s.floor = budget;
+        paged_release(c, s, keep);
+    }
+    return MNI_OK;
+}
+static int paged_track(PagedCache &c, const uint32_t *seqs, size_t n, uint32_t *weights, uint32_t *positions) {
+    const PagedPool &p = c.pool;
+    if (!p.weight) return set_error(MNI_ERR_INVALID, "paged cache track: the cache is not tracked");
+    MNI_TRY(paged_check(c, seqs, n, false, "track"));
+    const int64_t width = paged_longest(c, seqs, n), total = (int64_t)n * p.heads * width;
+    BufP w = new_buf((size_t)total);
+    IntBuf pos;
+    pos.data = w ? dev_ints((size_t)total) : nullptr;
+    if (!pos.data) return MNI_ERR_NOMEM;
+    pos.len = total;
+    pos.lo = -1;
+    pos.hi = INT32_MAX;
+    for (size_t first = 0; first < n; first += PAGED_BATCH) {
+        const int64_t at = (int64_t)first * p.heads * width;
+        MNI_TRY(k_paged_track(p, paged_batch(c, seqs, first, n), w->p + at, (int32_t *)pos.data.get() + at, width));
+    }
+    *weights = insert_contig(std::move(w), Shape{(int64_t)n, p.heads, width});
+    *positions = insert_int(std::move(pos));
+    return MNI_OK;
+}
+static int paged_read(PagedCache &c, uint32_t seq, uint32_t *out_ids) {
+    PagedSequence *s = paged_seq(c, seq);
+    if (!s) return MNI_ERR_INVALID;
+    const PagedPool &p = c.pool;
+    const Shape shape{p.heads, s->len, p.d};
+    BufP k = new_buf((size_t)(p.heads * s->len * p.d)), v = k ? new_buf((size_t)(p.heads * s->len * p.d)) : nullptr;
+    if (!v) return MNI_ERR_NOMEM;
+    MNI_TRY(k_paged_read(p, (int32_t)seq, s->len, k->p, v->p));
+    out_ids[0] = insert_contig(std::move(k), shape);
+    out_ids[1] = insert_contig(std::move(v), shape);
+    return MNI_OK;
+}
+
 // ops/mixed_precision.rs:17-32: grads *= inv_scale, true when any scaled value is inf or NaN
 static int scale_grads_checked(const uint32_t *ids, size_t n, float inv_scale, int *found) {
     BufP flag = new_buf(1);
@@ -1858,6 +2326,7 @@ static int dispatch_backward(const Entry &e, uint32_t grad, int64_t *out) {  // 
     case OP_DROPOUT: return dropout_backward(grad, e, out);
     case OP_RESIDUALLAYERNORM: return residual_layernorm_backward(grad, e, out);
     case OP_MSEROWS: return mse_rows_backward(grad, e, out);
+    case OP_NORMROPE: return norm_rope_backward(grad, e, out);
     }
     return set_error(MNI_ERR_INVALID, "unknown tape op %d", e.op);
 }
@@ -2201,6 +2670,17 @@ using namespace mni;
 // ============================================================================
 // Exported engine surface (one function per #[napi] export of lib.rs)
 // ============================================================================
+// Lists of the host grow with a caller's arguments: running out of memory for them is an error, not an abort.
+template <class F>
+static auto guarded(F f, decltype(f()) failed) -> decltype(f()) {
+    try {
+        return f();
+    } catch (const std::exception &e) {
+        set_error(MNI_ERR_NOMEM, "out of host memory: %s", e.what());
+        return failed;
+    }
+}
+
 extern "C" {
 
 uint32_t mni_zeros(const int64_t *shape, int ndim) {
@@ -2468,6 +2948,8 @@ void mni_reset_engine(void) {
     e.tape = Tape();
     e.kv_caches.clear();       // lib.rs:466-467
     e.next_kv_cache_id = 1;
+    e.paged_caches.clear();
+    e.next_paged_cache_id = 1;
     e.int_bufs.clear();        // lib.rs:465
     e.int_free.clear();
 }
@@ -2579,6 +3061,99 @@ uint32_t mni_tile(uint32_t input, const int64_t *reps, int n) {  // lib.rs:568-5
     MNI_API_GUARD;
     if (n > 0 && !reps) { set_error(MNI_ERR_INVALID, "tile: null reps"); return MNI_BAD_ID; }
     return tile_op(input, reps, n);
+}
+
+// ---- norm and rotation, paged KV cache ------------------------------------------------------
+int mni_qk_norm_rope(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k, uint32_t positions, int64_t offset, int64_t rotary_dims,
+                     int interleaved, double theta, double eps, uint32_t *out_ids) {
+    MNI_API_GUARD;
+    if (!out_ids) return set_error(MNI_ERR_INVALID, "qk_norm_rope: null out_ids");
+    return guarded([&] { return norm_rope_op(q, k, gamma_q, gamma_k, positions, offset, rotary_dims, interleaved, theta, eps, out_ids); }, MNI_ERR_NOMEM);
+}
+uint32_t mni_paged_cache_create(int64_t max_sequences, int64_t max_seq_len, int64_t num_pages, int64_t page_size, int64_t kv_heads, int64_t head_dim,
+                                int quantized, int tracked) {
+    MNI_API_GUARD;
+    return guarded([&] { return paged_create(max_sequences, max_seq_len, num_pages, page_size, kv_heads, head_dim, quantized != 0, tracked != 0); }, MNI_BAD_ID);
+}
+void mni_paged_cache_free(uint32_t cache_id) { MNI_API_GUARD; eng().paged_caches.erase(cache_id); }
+int64_t mni_paged_cache_free_pages(uint32_t cache_id) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    return c ? (int64_t)c->free_pages.size() : -1;
+}
+uint32_t mni_paged_cache_add(uint32_t cache_id) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    return c ? paged_add(*c) : MNI_BAD_ID;
+}
+uint32_t mni_paged_cache_fork(uint32_t cache_id, uint32_t seq) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    return c ? guarded([&] { return paged_fork(*c, seq); }, MNI_BAD_ID) : MNI_BAD_ID;
+}
+int mni_paged_cache_drop(uint32_t cache_id, uint32_t seq) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    PagedSequence *s = c ? paged_seq(*c, seq) : nullptr;
+    if (!s) return MNI_ERR_INVALID;
+    paged_release(*c, *s, 0);
+    *s = PagedSequence();
+    c->free_seqs.push_back(seq);
+    return MNI_OK;
+}
+int64_t mni_paged_cache_len(uint32_t cache_id, uint32_t seq) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    PagedSequence *s = c ? paged_seq(*c, seq) : nullptr;
+    return s ? s->len : -1;
+}
+int64_t mni_paged_cache_seen(uint32_t cache_id, uint32_t seq) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    PagedSequence *s = c ? paged_seq(*c, seq) : nullptr;
+    return s ? s->seen : -1;
+}
+int mni_paged_cache_append(uint32_t cache_id, const uint32_t *seqs, size_t n, uint32_t k, uint32_t v, const int64_t *counts) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    return c ? guarded([&] { return paged_append(*c, seqs, n, k, v, counts); }, MNI_ERR_NOMEM) : MNI_ERR_INVALID;
+}
+int mni_paged_cache_truncate(uint32_t cache_id, const uint32_t *seqs, size_t n, const int64_t *lens) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    return c ? guarded([&] { return paged_truncate(*c, seqs, n, lens); }, MNI_ERR_NOMEM) : MNI_ERR_INVALID;
+}
+uint32_t mni_paged_cache_attend(uint32_t cache_id, const uint32_t *seqs, size_t n, uint32_t q, double scale, int accumulate) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    return c ? guarded([&] { return paged_attend(*c, seqs, n, q, (float)scale, accumulate != 0); }, MNI_BAD_ID) : MNI_BAD_ID;
+}
+int mni_paged_cache_add_weights(uint32_t cache_id, const uint32_t *seqs, size_t n, uint32_t w) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    return c ? guarded([&] { return paged_add_weights(*c, seqs, n, w); }, MNI_ERR_NOMEM) : MNI_ERR_INVALID;
+}
+int mni_paged_cache_evict(uint32_t cache_id, const uint32_t *seqs, size_t n, int64_t budget, int64_t recent) {
+    MNI_API_GUARD;
+    PagedCache *c = paged(cache_id);
+    return c ? guarded([&] { return paged_evict(*c, seqs, n, budget, recent); }, MNI_ERR_NOMEM) : MNI_ERR_INVALID;
+}
+int mni_paged_cache_track(uint32_t cache_id, const uint32_t *seqs, size_t n, uint32_t *weights, uint32_t *positions) {
+    MNI_API_GUARD;
+    if (!weights || !positions) return set_error(MNI_ERR_INVALID, "paged cache track: null output");
+    PagedCache *c = paged(cache_id);
+    return c ? guarded([&] { return paged_track(*c, seqs, n, weights, positions); }, MNI_ERR_NOMEM) : MNI_ERR_INVALID;
+}
+int mni_paged_cache_read(uint32_t cache_id, uint32_t seq, uint32_t *out_ids) {
+    MNI_API_GUARD;
+    if (!out_ids) return set_error(MNI_ERR_INVALID, "paged cache read: null output");
+    PagedCache *c = paged(cache_id);
+    return c ? guarded([&] { return paged_read(*c, seq, out_ids); }, MNI_ERR_NOMEM) : MNI_ERR_INVALID;
+}
+void *mni_rocm_int_buffer_ptr(uint32_t id) {
+    MNI_API_GUARD;
+    IntBuf *b = get_int(id);
+    return b ? b->data.get() : nullptr;
 }
 
 void *mni_dev_ptr(uint32_t id) {

@@ -39,8 +39,8 @@ napi_value ret_id(napi_env env, uint32_t id) { return id == MNI_BAD_ID ? throw_l
 napi_value ret_rc(napi_env env, int rc) { return rc != MNI_OK ? throw_last(env) : undefined(env); }
 
 struct Args {
-    napi_value v[9];
-    size_t n = 9;
+    napi_value v[10];
+    size_t n = 10;
     Args(napi_env env, napi_callback_info info) { napi_get_cb_info(env, info, &n, v, nullptr, nullptr); }
 };
 uint32_t get_u32(napi_env env, napi_value v) {
@@ -299,6 +299,111 @@ napi_value KvCacheDecodeStep(napi_env env, napi_callback_info info) {  // lib.rs
     return ret_id(env, mni_kv_cache_decode_step(get_u32(env, a.v[0]), get_u32(env, a.v[1]), get_u32(env, a.v[2]),
                                                 get_u32(env, a.v[3]), get_f64(env, a.v[4])));
 }
+// Norm + rotation and the paged cache (no counterparts in lib.rs; feature-detected by callers).
+napi_value ret_ids(napi_env env, int rc, uint32_t first, uint32_t second) {
+    if (rc != MNI_OK) return throw_last(env);
+    napi_value arr;
+    napi_create_array_with_length(env, 2, &arr);
+    napi_set_element(env, arr, 0, make_u32(env, first));
+    napi_set_element(env, arr, 1, make_u32(env, second));
+    return arr;
+}
+bool is_given(napi_env env, napi_value v) {  // neither undefined nor null
+    napi_valuetype t;
+    return napi_typeof(env, v, &t) == napi_ok && t != napi_undefined && t != napi_null;
+}
+napi_value QkNormRope(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    uint32_t out[2] = {0, 0};
+    const int rc = mni_qk_norm_rope(get_u32(env, a.v[0]), get_u32(env, a.v[1]), get_u32(env, a.v[2]), get_u32(env, a.v[3]),
+                                    is_given(env, a.v[4]) ? get_u32(env, a.v[4]) : MNI_BAD_ID, get_i64(env, a.v[5]), get_i64(env, a.v[6]),
+                                    get_bool(env, a.v[7]) ? 1 : 0, get_f64(env, a.v[8]), get_f64(env, a.v[9]), out);
+    return ret_ids(env, rc, out[0], out[1]);
+}
+napi_value PagedCacheCreate(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    return ret_id(env, mni_paged_cache_create(get_i64(env, a.v[0]), get_i64(env, a.v[1]), get_i64(env, a.v[2]), get_i64(env, a.v[3]), get_i64(env, a.v[4]),
+                                              get_i64(env, a.v[5]), get_bool(env, a.v[6]) ? 1 : 0, get_bool(env, a.v[7]) ? 1 : 0));
+}
+napi_value PagedCacheFree(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    mni_paged_cache_free(get_u32(env, a.v[0]));
+    return undefined(env);
+}
+napi_value ret_count(napi_env env, int64_t n) { return n < 0 ? throw_last(env) : make_f64(env, (double)n); }
+napi_value PagedCacheFreePages(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    return ret_count(env, mni_paged_cache_free_pages(get_u32(env, a.v[0])));
+}
+napi_value PagedCacheAdd(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    return ret_id(env, mni_paged_cache_add(get_u32(env, a.v[0])));
+}
+napi_value PagedCacheFork(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    return ret_id(env, mni_paged_cache_fork(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
+}
+napi_value PagedCacheDrop(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    return ret_rc(env, mni_paged_cache_drop(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
+}
+napi_value PagedCacheLen(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    return ret_count(env, mni_paged_cache_len(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
+}
+napi_value PagedCacheSeen(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    return ret_count(env, mni_paged_cache_seen(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
+}
+napi_value throw_lengths(napi_env env, const char *what) {
+    napi_throw_error(env, nullptr, what);
+    return nullptr;
+}
+napi_value PagedCacheAppend(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    const bool some = is_given(env, a.v[4]);
+    const std::vector<int64_t> counts = some ? get_i64_array(env, a.v[4]) : std::vector<int64_t>();
+    if (some && counts.size() != seqs.size()) return throw_lengths(env, "paged cache append: as many counts as sequences are wanted");
+    return ret_rc(env, mni_paged_cache_append(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2]), get_u32(env, a.v[3]),
+                                              some ? counts.data() : nullptr));
+}
+napi_value PagedCacheTruncate(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    const std::vector<int64_t> lens = get_i64_array(env, a.v[2]);
+    if (lens.size() != seqs.size()) return throw_lengths(env, "paged cache truncate: as many lengths as sequences are wanted");
+    return ret_rc(env, mni_paged_cache_truncate(get_u32(env, a.v[0]), seqs.data(), seqs.size(), lens.data()));
+}
+napi_value PagedCacheAttend(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    return ret_id(env, mni_paged_cache_attend(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2]), get_f64(env, a.v[3]),
+                                              get_bool(env, a.v[4]) ? 1 : 0));
+}
+napi_value PagedCacheAddWeights(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    return ret_rc(env, mni_paged_cache_add_weights(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2])));
+}
+napi_value PagedCacheEvict(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    return ret_rc(env, mni_paged_cache_evict(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_i64(env, a.v[2]), get_i64(env, a.v[3])));
+}
+napi_value PagedCacheTrack(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    uint32_t w = 0, p = 0;
+    const int rc = mni_paged_cache_track(get_u32(env, a.v[0]), seqs.data(), seqs.size(), &w, &p);
+    return ret_ids(env, rc, w, p);
+}
+napi_value PagedCacheRead(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    uint32_t out[2] = {0, 0};
+    const int rc = mni_paged_cache_read(get_u32(env, a.v[0]), get_u32(env, a.v[1]), out);
+    return ret_ids(env, rc, out[0], out[1]);
+}
 napi_value PowOp(napi_env env, napi_callback_info info) {  // lib.rs:381-386
     Args a(env, info);
     return ret_id(env, mni_pow_op(get_u32(env, a.v[0]), get_f64(env, a.v[1])));
@@ -434,6 +539,12 @@ NAPI_MODULE_INIT() {
         EXPORT("kvCacheCreate", KvCacheCreate), EXPORT("kvCacheLen", KvCacheLen), EXPORT("kvCacheQuantized", KvCacheQuantized),
         EXPORT("kvCacheReset", KvCacheReset), EXPORT("kvCacheFree", KvCacheFree), EXPORT("kvCacheAppend", KvCacheAppend),
         EXPORT("kvCacheDecodeStep", KvCacheDecodeStep), EXPORT("flashAttention", FlashAttention),
+        EXPORT("qkNormRope", QkNormRope), EXPORT("pagedCacheCreate", PagedCacheCreate), EXPORT("pagedCacheFree", PagedCacheFree),
+        EXPORT("pagedCacheFreePages", PagedCacheFreePages), EXPORT("pagedCacheAdd", PagedCacheAdd), EXPORT("pagedCacheFork", PagedCacheFork),
+        EXPORT("pagedCacheDrop", PagedCacheDrop), EXPORT("pagedCacheLen", PagedCacheLen), EXPORT("pagedCacheSeen", PagedCacheSeen),
+        EXPORT("pagedCacheAppend", PagedCacheAppend), EXPORT("pagedCacheTruncate", PagedCacheTruncate), EXPORT("pagedCacheAttend", PagedCacheAttend),
+        EXPORT("pagedCacheAddWeights", PagedCacheAddWeights), EXPORT("pagedCacheEvict", PagedCacheEvict), EXPORT("pagedCacheTrack", PagedCacheTrack),
+        EXPORT("pagedCacheRead", PagedCacheRead),
         EXPORT("randTensor", RandTensor), EXPORT("randnTensor", RandnTensor), EXPORT("seed", Seed), EXPORT("philoxWords", PhiloxWords), EXPORT("tile", Tile),
         EXPORT("dropoutOp", DropoutOp), EXPORT("createDataset", CreateDataset), EXPORT("sampleBatch", SampleBatch),
         EXPORT("freeIntBuffer", FreeIntBuffer), EXPORT("intBufferToInt32", IntBufferToInt32),

@@ -47,6 +47,18 @@ class GemmDesc(C.Structure):
                 ("split_k", C.c_int32), ("algo", C.c_int32), ("aux", C.c_void_p), ("colsum_part", C.c_void_p)]
 
 
+class RopeHeads(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("heads", C.c_int64), ("batch_stride", C.c_int64), ("head_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("gamma", C.c_void_p), ("out", C.c_void_p), ("grad", C.c_void_p), ("dx", C.c_void_p), ("dgamma", C.c_void_p)]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("seq", C.c_int64), ("head_dim", C.c_int64), ("rotary_dims", C.c_int64),
+                ("positions", C.c_void_p), ("position_stride", C.c_int64), ("offset", C.c_int64),
+                ("theta", C.c_double), ("eps", C.c_double), ("interleaved", C.c_int32), ("reserved", C.c_int32),
+                ("q", RopeHeads), ("k", RopeHeads)]
+
+
 # name -> (restype, argtypes): every symbol include/mni_rocm.h declares.
 SIGNATURES = {
     "mni_rocm_init": (C.c_int, [C.c_int]),
@@ -83,6 +95,8 @@ SIGNATURES = {
     "mni_rocm_unbroadcast": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_int64), C.c_int]),
     "mni_rocm_axpy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_float, C.c_int64]),
     "mni_rocm_fill": (C.c_int, [C.c_void_p, C.c_float, C.c_int64]),
+    "mni_rocm_qk_norm_rope": (C.c_int, [C.POINTER(RopeDesc)]),
+    "mni_rocm_qk_norm_rope_backward": (C.c_int, [C.POINTER(RopeDesc)]),
     "mni_zeros": (C.c_uint32, [_i64p, C.c_int]),
     "mni_ones": (C.c_uint32, [_i64p, C.c_int]),
     "mni_from_float32": (C.c_uint32, [C.c_void_p, C.c_size_t, _i64p, C.c_int]),
@@ -150,7 +164,21 @@ SIGNATURES = {
     "mni_gc_tensors": (C.c_int, [_u32p, C.c_size_t]),
     "mni_linear": (C.c_uint32, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_int]),
     "mni_mse_loss": (C.c_uint32, [C.c_uint32, C.c_uint32]),
+    "mni_qk_norm_rope": (C.c_int, [C.c_uint32] * 5 + [C.c_int64, C.c_int64, C.c_int, C.c_double, C.c_double, _u32p]),
+    "mni_paged_cache_create": (C.c_uint32, [C.c_int64] * 6 + [C.c_int, C.c_int]),
+    "mni_paged_cache_free": (None, [C.c_uint32]), "mni_paged_cache_free_pages": (C.c_int64, [C.c_uint32]),
+    "mni_paged_cache_add": (C.c_uint32, [C.c_uint32]), "mni_paged_cache_fork": (C.c_uint32, [C.c_uint32] * 2),
+    "mni_paged_cache_drop": (C.c_int, [C.c_uint32] * 2),
+    "mni_paged_cache_len": (C.c_int64, [C.c_uint32] * 2), "mni_paged_cache_seen": (C.c_int64, [C.c_uint32] * 2),
+    "mni_paged_cache_append": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, C.c_uint32, C.c_uint32, _i64p]),
+    "mni_paged_cache_truncate": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, _i64p]),
+    "mni_paged_cache_attend": (C.c_uint32, [C.c_uint32, _u32p, C.c_size_t, C.c_uint32, C.c_double, C.c_int]),
+    "mni_paged_cache_add_weights": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, C.c_uint32]),
+    "mni_paged_cache_evict": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, C.c_int64, C.c_int64]),
+    "mni_paged_cache_track": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, _u32p, _u32p]),
+    "mni_paged_cache_read": (C.c_int, [C.c_uint32, C.c_uint32, _u32p]),
     "mni_dev_ptr": (C.c_void_p, [C.c_uint32]),
+    "mni_rocm_int_buffer_ptr": (C.c_void_p, [C.c_uint32]),
 }
 
 _lib = None
@@ -353,6 +381,26 @@ class Rocm:
     def fill(self, dst, value, n):
         self._check(self.lib.mni_rocm_fill(dst, value, n))
 
+    @staticmethod
+    def rope_desc(q, k=None, *, batch, seq, head_dim, rotary_dims=None, positions=None, position_stride=0, offset=0, interleaved=False,
+                  theta=10000.0, eps=1e-6):
+        """q, k: dicts of device addresses x, gamma and out (forward) or grad, dx and dgamma (backward), `heads`, and
+        `strides` of x in elements (batch, head, token; default: x contiguous [batch, heads, seq, head_dim])."""
+        def heads(o):
+            if o is None:
+                return RopeHeads()
+            s = o.get("strides") or (o["heads"] * seq * head_dim, seq * head_dim, head_dim)
+            return RopeHeads(o["x"], o["heads"], s[0], s[1], s[2], o["gamma"], o.get("out"), o.get("grad"), o.get("dx"), o.get("dgamma"))
+        return RopeDesc(batch, seq, head_dim, head_dim if rotary_dims is None else rotary_dims, positions, position_stride, offset, theta, eps,
+                        1 if interleaved else 0, 0, heads(q), heads(k))
+
+    def qk_norm_rope(self, q, k=None, **plan):
+        """Norm of queries and keys for each head and the rotation of their positions, in one launch (see rope_desc)."""
+        self._check(self.lib.mni_rocm_qk_norm_rope(C.byref(self.rope_desc(q, k, **plan))))
+
+    def qk_norm_rope_backward(self, q, k=None, **plan):
+        self._check(self.lib.mni_rocm_qk_norm_rope_backward(C.byref(self.rope_desc(q, k, **plan))))
+
 
 class Native:
     """Engine-level ABI under the reference's N-API export names."""
@@ -513,6 +561,71 @@ class Native:
     def kvCacheDecodeStep(self, cacheId, q, k, v, scale):
         return self._id(self.lib.mni_kv_cache_decode_step(cacheId, q, k, v, scale))
 
+    def qkNormRope(self, q, k, gammaQ, gammaK, positions, offset, rotaryDims, interleaved, theta, eps):
+        out = (C.c_uint32 * 2)()
+        self._rc(self.lib.mni_qk_norm_rope(q, k, gammaQ, gammaK, BAD_ID if positions is None else positions, offset, rotaryDims,
+                                           1 if interleaved else 0, theta, eps, out))
+        return [int(out[0]), int(out[1])]
+
+    def pagedCacheCreate(self, maxSequences, maxSeqLen, numPages, pageSize, numKvHeads, headDim, quantized, tracked):
+        return self._id(self.lib.mni_paged_cache_create(maxSequences, maxSeqLen, numPages, pageSize, numKvHeads, headDim, 1 if quantized else 0,
+                                                        1 if tracked else 0))
+
+    def pagedCacheFree(self, cacheId):
+        self.lib.mni_paged_cache_free(cacheId)
+
+    def _count(self, v):
+        if v < 0:
+            raise self._err()
+        return int(v)
+
+    def pagedCacheFreePages(self, cacheId):
+        return self._count(self.lib.mni_paged_cache_free_pages(cacheId))
+
+    def pagedCacheAdd(self, cacheId):
+        return self._id(self.lib.mni_paged_cache_add(cacheId))
+
+    def pagedCacheFork(self, cacheId, seq):
+        return self._id(self.lib.mni_paged_cache_fork(cacheId, seq))
+
+    def pagedCacheDrop(self, cacheId, seq):
+        self._rc(self.lib.mni_paged_cache_drop(cacheId, seq))
+
+    def pagedCacheLen(self, cacheId, seq):
+        return self._count(self.lib.mni_paged_cache_len(cacheId, seq))
+
+    def pagedCacheSeen(self, cacheId, seq):
+        return self._count(self.lib.mni_paged_cache_seen(cacheId, seq))
+
+    def pagedCacheAppend(self, cacheId, seqs, k, v, counts=None):
+        if counts is not None and len(counts) != len(seqs):
+            raise MniError("paged cache append: %d counts for %d sequences" % (len(counts), len(seqs)))
+        self._rc(self.lib.mni_paged_cache_append(cacheId, _u32_array(seqs), len(seqs), k, v, None if counts is None else _i64_array(counts)))
+
+    def pagedCacheTruncate(self, cacheId, seqs, lens):
+        if len(lens) != len(seqs):
+            raise MniError("paged cache truncate: %d lengths for %d sequences" % (len(lens), len(seqs)))
+        self._rc(self.lib.mni_paged_cache_truncate(cacheId, _u32_array(seqs), len(seqs), _i64_array(lens)))
+
+    def pagedCacheAttend(self, cacheId, seqs, q, scale, accumulate):
+        return self._id(self.lib.mni_paged_cache_attend(cacheId, _u32_array(seqs), len(seqs), q, scale, 1 if accumulate else 0))
+
+    def pagedCacheAddWeights(self, cacheId, seqs, w):
+        self._rc(self.lib.mni_paged_cache_add_weights(cacheId, _u32_array(seqs), len(seqs), w))
+
+    def pagedCacheEvict(self, cacheId, seqs, budget, recent):
+        self._rc(self.lib.mni_paged_cache_evict(cacheId, _u32_array(seqs), len(seqs), budget, recent))
+
+    def pagedCacheTrack(self, cacheId, seqs):
+        w, p = C.c_uint32(0), C.c_uint32(0)
+        self._rc(self.lib.mni_paged_cache_track(cacheId, _u32_array(seqs), len(seqs), C.byref(w), C.byref(p)))
+        return [w.value, p.value]
+
+    def pagedCacheRead(self, cacheId, seq):
+        out = (C.c_uint32 * 2)()
+        self._rc(self.lib.mni_paged_cache_read(cacheId, seq, out))
+        return [int(out[0]), int(out[1])]
+
     def expOp(self, a):
         return self._id(self.lib.mni_exp_op(a))
 
@@ -639,6 +752,12 @@ class Native:
 
     def devPtr(self, id):
         p = self.lib.mni_dev_ptr(id)
+        if not p:
+            raise self._err()
+        return p
+
+    def intBufferPtr(self, id):
+        p = self.lib.mni_rocm_int_buffer_ptr(id)
         if not p:
             raise self._err()
         return p

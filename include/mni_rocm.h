@@ -254,6 +254,42 @@ int mni_rocm_axpy(float *dst, const float *src, float alpha, int64_t n);
 /* dst[i] = value                  (fill_f32, src/native/src/tensor.rs:395-442) */
 int mni_rocm_fill(float *dst, float value, int64_t n);
 
+/* Norm of queries and keys for each head and the rotation of their positions, in one pass.  No counterpart in the
+ * reference, whose attention (src/native/src/ops/attention.rs:14-78) takes queries and keys as they come; the outputs
+ * are laid out as mni_flash_attention and the caches take them.  For every row x of head_dim values with its gain g:
+ *   r = 1 / sqrt(mean(x^2) + eps),  z = x r g,
+ *   y[lo] = z[lo] cos a - z[hi] sin a,  y[hi] = z[hi] cos a + z[lo] sin a,  the values from rotary_dims on unrotated,
+ * with a = (position + offset) * theta^(-2 i / rotary_dims) for pair i = 0 .. rotary_dims / 2 - 1, which is (i, i +
+ * rotary_dims / 2), or (2i, 2i + 1) when `interleaved`.  Angles are formed in 64 bits and reduced to a fraction of a
+ * turn before the 32-bit sine and cosine, so a far position is as exact as a near one.
+ * `heads` rows per token, x[b, h, s, :] = x + b * batch_stride + h * head_stride + s * token_stride (elements, the
+ * last extent contiguous: a projection's output, or its part of a fused one, is read where it lies); outputs
+ * contiguous [batch, heads, seq, head_dim].  heads == 0 leaves that operand out.
+ * positions: seq int32 values, of sequence b at positions + b * position_stride (0: shared by all); NULL: 0 .. seq - 1.
+ * Errors: head_dim not in 1 .. 256, rotary_dims odd, negative or beyond head_dim, theta or eps not positive
+ * (eps may be 0). */
+typedef struct {
+    const float *x;
+    int64_t heads, batch_stride, head_stride, token_stride;
+    const float *gamma;  /* head_dim gains */
+    float *out;          /* forward */
+    const float *grad;   /* backward: d loss / d out, laid out like out */
+    float *dx;           /* backward: [batch, heads, seq, head_dim], contiguous */
+    float *dgamma;       /* backward: head_dim values, overwritten */
+} mni_rope_heads;
+typedef struct {
+    int64_t batch, seq, head_dim, rotary_dims;
+    const int32_t *positions;
+    int64_t position_stride, offset;
+    double theta, eps;
+    int32_t interleaved, reserved;
+    mni_rope_heads q, k;
+} mni_rope_desc;
+int mni_rocm_qk_norm_rope(const mni_rope_desc *desc);
+/* Its backward.  With dz the gradient rotated back: dx = r dz g - x r^3 mean(dz g x) and dgamma = the sum over all
+ * rows of dz x r, each taken in a fixed order (the same bits every time).  `out` is not read. */
+int mni_rocm_qk_norm_rope_backward(const mni_rope_desc *desc);
+
 /* ------------------------------------------------------------------------- *
  * 2. Engine level: mirrors src/native/src/lib.rs export by export.
  * ------------------------------------------------------------------------- */
@@ -404,9 +440,67 @@ uint32_t mni_linear(uint32_t x, uint32_t w, uint32_t bias, int act);
  * mni_linear. */
 uint32_t mni_mse_loss(uint32_t pred, uint32_t target);
 
+/* Norm and rotation of queries [B, Hq, S, D] and keys [B, Hk, S, D] (views welcome: the [B, S, H, D] output of a
+ * projection seen through permute is read where it lies) before attention or a cache, in one pass: see
+ * mni_rocm_qk_norm_rope.  gamma_q, gamma_k: [D].  positions: an int buffer of S or B * S values, or MNI_BAD_ID for
+ * 0 .. S - 1; `offset` is added to each.  out_ids[0..1] = the rotated queries and keys, contiguous; both are recorded
+ * on the tape, whose backward yields the gradients of q, k and the gains.  No counterpart in the reference. */
+int mni_qk_norm_rope(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k, uint32_t positions, int64_t offset,
+                     int64_t rotary_dims, int interleaved, double theta, double eps, uint32_t *out_ids);
+
+/* Paged key-value cache: sequences of different lengths share one pool of pages of `page_size` positions each, so
+ * memory goes by the tokens held.  Next to mni_kv_cache_* (the reference's cache: one fixed batch, all of one length,
+ * src/native/src/ops/kv_cache.rs:20-47); rows are stored as that one stores them, fp32 or int8 with one f32 scale per
+ * row.  No counterpart in the reference.  Ids of caches start at 1 and restart after mni_reset_engine; sequence ids
+ * are recycled, the last freed first.  kv_heads may be fewer than the queries' heads (a divisor: query head h reads
+ * key head h / (heads / kv_heads)).
+ * create: max_sequences sequences of at most max_seq_len tokens; num_pages pages of page_size positions (a power of
+ *   two up to 1024); head_dim up to 256.  `tracked`: the cache also keeps, for every position and key head, an
+ *   accumulated attention weight and the position that the row was appended at, which eviction goes by.
+ * add: a new, empty sequence.  fork: one that starts as a copy of seq; pages are shared until one of the two writes
+ *   to them.  drop: frees a sequence and the pages that no other sequence holds.
+ * len: tokens held; seen: tokens appended less those truncated (the rotation position of the next one; eviction does
+ *   not change it); free_pages: pages that no sequence holds.  < 0 for an unknown id.
+ * append: k, v [n, kv_heads, T, head_dim] (views welcome): sequence seqs[i] takes its first counts[i] <= T tokens, or
+ *   all T where counts is NULL.  A sequence may not occur twice.
+ * truncate: back to lens[i] rows, the tokens appended last leave first (rejected drafts).  Of a sequence that has
+ *   been evicted only tokens appended since then can leave this way.
+ * attend: q [n, heads, 1, head_dim] (or [n * heads, 1, head_dim]) attends over everything seqs[i] holds: softmax(scale
+ *   q k^T) v, in q's shape; zeros where a sequence holds nothing.  `accumulate` (tracked caches): every position's
+ *   probability, summed over the query heads of its key head, is added to its weight; a sequence may then not occur
+ *   twice.
+ * add_weights: w [n, kv_heads, L], L at least the longest of them: w[i, h, j] is added to the weight of row j.
+ * evict: sequences of more than `budget` tokens are cut to `budget` rows per key head.  The rows of the last `recent`
+ *   tokens stay, then those of the largest weight, equal weights by the earlier position (a NaN counts as the
+ *   largest).  A row that stays below the budget keeps its place; the freed places take the surviving rows behind the
+ *   budget, in order, with their weights and positions.  Pages behind the budget are freed; pages shared with a fork
+ *   are copied first.
+ * track: the weights, as a tensor [n, kv_heads, longest], and the positions, as an int buffer of as many values, of
+ *   every row in the order held; 0 and -1 behind a sequence's end.
+ * read: keys and values of one sequence in the order held, [kv_heads, len, head_dim] (int8 rows as the values they
+ *   stand for). */
+uint32_t mni_paged_cache_create(int64_t max_sequences, int64_t max_seq_len, int64_t num_pages, int64_t page_size, int64_t kv_heads,
+                                int64_t head_dim, int quantized, int tracked);
+void mni_paged_cache_free(uint32_t cache_id);
+int64_t mni_paged_cache_free_pages(uint32_t cache_id);
+uint32_t mni_paged_cache_add(uint32_t cache_id);
+uint32_t mni_paged_cache_fork(uint32_t cache_id, uint32_t seq);
+int mni_paged_cache_drop(uint32_t cache_id, uint32_t seq);
+int64_t mni_paged_cache_len(uint32_t cache_id, uint32_t seq);
+int64_t mni_paged_cache_seen(uint32_t cache_id, uint32_t seq);
+int mni_paged_cache_append(uint32_t cache_id, const uint32_t *seqs, size_t n, uint32_t k, uint32_t v, const int64_t *counts);
+int mni_paged_cache_truncate(uint32_t cache_id, const uint32_t *seqs, size_t n, const int64_t *lens);
+uint32_t mni_paged_cache_attend(uint32_t cache_id, const uint32_t *seqs, size_t n, uint32_t q, double scale, int accumulate);
+int mni_paged_cache_add_weights(uint32_t cache_id, const uint32_t *seqs, size_t n, uint32_t w);
+int mni_paged_cache_evict(uint32_t cache_id, const uint32_t *seqs, size_t n, int64_t budget, int64_t recent);
+int mni_paged_cache_track(uint32_t cache_id, const uint32_t *seqs, size_t n, uint32_t *weights, uint32_t *positions);
+int mni_paged_cache_read(uint32_t cache_id, uint32_t seq, uint32_t *out_ids);
+
 /* Device address of a tensor's buffer (cuda arm: TensorStore::dev_ptr,
  * src/native/src/tensor.rs:358-361). NULL on error. */
 void *mni_dev_ptr(uint32_t id);
+/* The same for an int buffer: what mni_rocm_qk_norm_rope takes as positions. NULL on error. */
+void *mni_rocm_int_buffer_ptr(uint32_t id);
 
 /* ------------------------------------------------------------------------- *
  * Measurement and test hooks.  NOT part of the drop-in boundary: nothing the
