@@ -371,9 +371,15 @@ def _ints_seen_by_torch(buffer, shape):
     return torch.as_tensor(_OnDevice(native.intBufferPtr(buffer), shape, "<i4", lambda: native.freeIntBuffer(buffer)), device=DEVICE)
 
 
+_bound = []
+
+
 def _api():
-    import framework_amd
-    return framework_amd.api()
+    if not _bound:
+        from framework_amd.api import bind
+        from framework_amd.native import Native
+        _bound.append(bind(Native()))
+    return _bound[0]
 
 
 def _given(x):
