@@ -371,15 +371,12 @@ def _ints_seen_by_torch(buffer, shape):
     return torch.as_tensor(_OnDevice(native.intBufferPtr(buffer), shape, "<i4", lambda: native.freeIntBuffer(buffer)), device=DEVICE)
 
 
-_bound = []
-
-
 def _api():
-    if not _bound:
+    if not hasattr(_api, "bound"):
         from framework_amd.api import bind
         from framework_amd.native import Native
-        _bound.append(bind(Native()))
-    return _bound[0]
+        _api.bound = bind(Native())
+    return _api.bound
 
 
 def _given(x):
