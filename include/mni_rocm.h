@@ -450,8 +450,8 @@ int mni_qk_norm_rope(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k,
 
 /* Paged key-value cache: sequences of different lengths share one pool of pages of `page_size` positions each, so
  * memory goes by the tokens held.  Next to mni_kv_cache_* (the reference's cache: one fixed batch, all of one length,
- * src/native/src/ops/kv_cache.rs:20-47); rows are stored as that one stores them, fp32 or int8 with one f32 scale per
- * row.  No counterpart in the reference.  Ids of caches start at 1 and restart after mni_reset_engine; sequence ids
+ * src/native/src/ops/kv_cache.rs:20-47); rows are fp32 or int8 codes with one f32 scale per row, as there.  No
+ * counterpart in the reference.  Ids of caches start at 1 and restart after mni_reset_engine; sequence ids
  * are recycled, the last freed first.  kv_heads may be fewer than the queries' heads (a divisor: query head h reads
  * key head h / (heads / kv_heads)).
  * create: max_sequences sequences of at most max_seq_len tokens; num_pages pages of page_size positions (a power of

@@ -23,7 +23,7 @@ def _stored(x, quantized):
     x = np.asarray(x, np.float32)
     if not quantized:
         return x
-    scale = np.maximum(np.abs(x).max(-1, keepdims=True) / np.float32(127.0), np.float32(1e-8)).astype(np.float32)
+    scale = np.maximum(np.abs(x).max(-1, keepdims=True) * (np.float32(1.0) / np.float32(127.0)), np.float32(1e-8)).astype(np.float32)
     y = (x * (np.float32(1.0) / scale).astype(np.float32)).astype(np.float32).astype(np.float64)
     codes = np.clip(np.sign(y) * np.floor(np.abs(y) + 0.5), -127, 127).astype(np.float32)
     return (codes * scale).astype(np.float32)
