@@ -45,6 +45,12 @@ struct PagedCopies {
     int32_t from[PAGED_PAIRS / 2], to[PAGED_PAIRS / 2];
 };
 
+#ifdef __HIPCC__
+__device__ __forceinline__ int64_t row_of(const PagedPool &p, int page, int head, int slot) {
+    return ((int64_t)page * p.heads + head) * p.page + slot;
+}
+#endif
+
 int k_paged_table(const PagedPool &p, const PagedTableWrite &w);
 int k_paged_copy(const PagedPool &p, const PagedCopies &c);
 int k_paged_append(const PagedPool &p, const PagedNew &in, const PagedAppend &a);
