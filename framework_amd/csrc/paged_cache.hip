@@ -7,6 +7,7 @@ namespace mni {
 namespace {
 
 constexpr int TPB = 256;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // ---- table entries, page copies, forks -----------------------------------------------------------------------------
 __global__ __launch_bounds__(TPB) void paged_table_kernel(int32_t *__restrict__ table, const PagedTableWrite w) {
@@ -40,78 +41,84 @@ __global__ __launch_bounds__(TPB) void paged_fork_kernel(const PagedPool p, int 
 
 // ---- append --------------------------------------------------------------------------------------------------------
 // A group of LPR lanes stores one key row and its value row.  int8: scale = max(max|x| * (1 / 127), 1e-8), codes
-// round(x * (1 / scale)), halves away from zero, within -127 .. 127: a stored value is at most half a scale off.  (The
-// contiguous cache divides by 127; the two scales differ by one rounding at most.)  VEC: 4 values per lane, else one
+// round(x * (1 / scale)), halves away from zero: a stored value is at most half a scale off, and no code leaves -127 .. 127
+// (the largest is 127 to three roundings).  (The contiguous cache divides by 127; the two scales differ by one rounding.)  VEC: 4 values per lane, else one
 // value per lane and turn.
-template <bool Q8, bool VEC, int LPR>
-__device__ __forceinline__ void append_row(const float *__restrict__ src, void *cache, float *scales, int64_t row, int d, int l) {
-    constexpr int N = VEC ? 1 : 4;  // pieces per lane (d <= 256)
+template <bool VEC>
+struct AppendRow {
+    static constexpr int N = VEC ? 1 : 4;  // pieces per lane (d <= 256)
     float4 x[N];
-    float mx = 0.f;
+    __device__ __forceinline__ void load(const float *__restrict__ src, int d, int l) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (VEC) {
-            if (4 * l < d) x[j] = *reinterpret_cast<const float4 *>(src + 4 * l);
-        } else if (l + 64 * j < d) {
-            x[j].x = src[l + 64 * j];
+        for (int j = 0; j < N; ++j) {
+            x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (VEC) {
+                if (4 * l < d) x[j] = *reinterpret_cast<const float4 *>(src + 4 * l);
+            } else if (l + 64 * j < d) {
+                x[j].x = src[l + 64 * j];
+            }
         }
-        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))));
     }
-    if (!Q8) {
-        float *dst = (float *)cache + row * d;
+    template <bool Q8, int LPR>
+    __device__ __forceinline__ void store(void *cache, float *scales, int64_t row, int d, int l) const {
+        if (!Q8) {
+            float *dst = (float *)cache + row * d;
+            if (VEC) {
+                if (4 * l < d) *reinterpret_cast<float4 *>(dst + 4 * l) = x[0];
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (l + 64 * j < d) dst[l + 64 * j] = x[j].x;
+            }
+            return;
+        }
+        float mx = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))));
+        mx = lanes_max<LPR>(mx);
+        float scale = mx * (1.0f / 127.0f);
+        if (!(scale > 1e-8f)) scale = 1e-8f;
+        const float inv = 1.0f / scale;
+        auto code = [&](float v) { return (int)roundf(v * inv); };
+        signed char *dst = (signed char *)cache + row * d;
         if (VEC) {
-            if (4 * l < d) *reinterpret_cast<float4 *>(dst + 4 * l) = x[0];
+            if (4 * l < d)
+                *reinterpret_cast<uint32_t *>(dst + 4 * l) = (uint32_t)(code(x[0].x) & 255) | (uint32_t)(code(x[0].y) & 255) << 8 |
+                                                             (uint32_t)(code(x[0].z) & 255) << 16 | (uint32_t)(code(x[0].w) & 255) << 24;
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (l + 64 * j < d) dst[l + 64 * j] = x[j].x;
+                if (l + 64 * j < d) dst[l + 64 * j] = (signed char)code(x[j].x);
         }
-        return;
+        if (l == 0) scales[row] = scale;
     }
-    mx = lanes_max<LPR>(mx);
-    float scale = mx * (1.0f / 127.0f);
-    if (!(scale > 1e-8f)) scale = 1e-8f;
-    const float inv = 1.0f / scale;
-    auto code = [&](float v) {
-        float q = roundf(v * inv);
-        q = q < -127.0f ? -127.0f : q > 127.0f ? 127.0f : q;
-        return (int)q;
-    };
-    signed char *dst = (signed char *)cache + row * d;
-    if (VEC) {
-        if (4 * l < d)
-            *reinterpret_cast<uint32_t *>(dst + 4 * l) = (uint32_t)(code(x[0].x) & 255) | (uint32_t)(code(x[0].y) & 255) << 8 |
-                                                         (uint32_t)(code(x[0].z) & 255) << 16 | (uint32_t)(code(x[0].w) & 255) << 24;
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (l + 64 * j < d) dst[l + 64 * j] = (signed char)code(x[j].x);
+};
+template <bool Q8, bool VEC, int LPR>
+__device__ __forceinline__ void append_store(const PagedPool &p, const PagedAppend &a, const AppendRow<VEC> &k, const AppendRow<VEC> &v, int page, int i, int h,
+                                             int t, int l) {
+    const int64_t at = (int64_t)a.len[i] + t, row = row_of(p, page, h, (int)(at & (p.page - 1)));
+    k.template store<Q8, LPR>(p.k, p.kscale, row, p.d, l);
+    v.template store<Q8, LPR>(p.v, p.vscale, row, p.d, l);
+    if (l == 0 && p.weight) {
+        const int64_t track = ((int64_t)a.slot[i] * p.heads + h) * p.max_len + at;
+        p.weight[track] = 0.f;
+        p.pos[track] = a.seen[i] + t;
     }
-    if (l == 0) scales[row] = scale;
 }
+// (Four rows a group, for prompts, measured no better: fp32 43.5 against 45 us on 134 MB, int8 14.3 against 11.3 on 29 MB.)
 template <bool Q8, bool VEC, int LPR>
 __global__ __launch_bounds__(TPB) void paged_append_kernel(const PagedPool p, const PagedNew in, const PagedAppend a) {
     const uint32_t idx = blockIdx.x * (TPB / LPR) + threadIdx.x / LPR;
     const uint32_t ih = idx / (uint32_t)in.tokens, t = idx - ih * in.tokens;
     const uint32_t i = ih / (uint32_t)p.heads, h = ih - i * p.heads;
     if (i >= (uint32_t)a.n || t >= (uint32_t)a.count[i]) return;  // (whole groups leave)
-    const int l = threadIdx.x % LPR;
-    const int64_t at = (int64_t)a.len[i] + t;
-    int32_t *entry = p.table + a.slot[i] * p.max_pages + (at >> p.shift);
-    const int fresh = a.page[i];
-    const int page = fresh >= 0 ? fresh : *entry;
-    const int64_t row = row_of(p, page, h, (int)(at & (p.page - 1)));
-    append_row<Q8, VEC, LPR>(in.k + i * in.k_seq + h * in.k_head + t * in.k_token, p.k, p.kscale, row, p.d, l);
-    append_row<Q8, VEC, LPR>(in.v + i * in.v_seq + h * in.v_head + t * in.v_token, p.v, p.vscale, row, p.d, l);
-    if (l == 0) {
-        if (fresh >= 0 && h == 0) *entry = fresh;
-        if (p.weight) {
-            const int64_t track = ((int64_t)a.slot[i] * p.heads + h) * p.max_len + at;
-            p.weight[track] = 0.f;
-            p.pos[track] = a.seen[i] + (int)t;
-        }
-    }
+    const int l = threadIdx.x % LPR, fresh = a.page[i];
+    int32_t *entry = p.table + a.slot[i] * p.max_pages + (((int64_t)a.len[i] + t) >> p.shift);
+    AppendRow<VEC> k, v;
+    k.load(in.k + i * in.k_seq + h * in.k_head + t * in.k_token, p.d, l);
+    v.load(in.v + i * in.v_seq + h * in.v_head + t * in.v_token, p.d, l);
+    append_store<Q8, VEC, LPR>(p, a, k, v, fresh >= 0 ? fresh : *entry, i, h, t, l);
+    if (fresh >= 0 && h == 0 && l == 0) *entry = fresh;
 }
 
 // ---- weights and positions -----------------------------------------------------------------------------------------
@@ -143,12 +150,16 @@ __global__ __launch_bounds__(TPB) void paged_read_kernel(const PagedPool p, int 
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------------
-// One workgroup per (sequence, key head) finds the rows that stay.  They are the `budget` first by (recent tokens,
-// weight, earlier position): a radix select on the weight as an ordered 32-bit key (recent rows above every key)
-// finds the last key that stays, eight bits a pass; where only some of the rows with that key stay, a second select on
-// the position tells which.  Then one pass in row order lists the freed places below the budget and the surviving rows
-// behind it, and paged_move_kernel moves row j of the second list to place j of the first.  No row is both read and
-// written, so the move needs no order and no second buffer, and it touches only what has to change place.
+// One workgroup per (sequence, key head) finds the rows that stay: the `budget` first by (recent tokens, weight, earlier
+// position).  The weight becomes an ordered 32-bit key (recent rows above every key), and the last key that stays is found
+// by its digits of eight bits from the highest on, each from a histogram of the keys that share the digits before; where
+// only some of the rows with that key stay, the same search on the position tells which.  A thread holds its keys in
+// registers (up to 32768 rows; of longer sequences they are read again, from the L2), every digit has a histogram of its
+// own, cleared at the start, and every wavefront reads it for itself: one barrier a digit.  (Two bits a turn by ballots, with
+// nothing to collide on, took 35 us on 256 x 4608 rows.)  Then one pass in row order lists the freed places below the
+// budget and the surviving rows behind it, and paged_move_kernel moves row j of the second list to place j of the first.
+// No row is both read and written, so the move needs no order and no second buffer, and it touches only what has to
+// change place.
 constexpr int SELECT_TPB = 1024;
 struct EvictArgs {
     PagedPool p;
@@ -157,15 +168,15 @@ struct EvictArgs {
     int32_t slot[PAGED_BATCH], len[PAGED_BATCH], seen[PAGED_BATCH];
 };
 __device__ __forceinline__ uint32_t weight_key(float w, bool recent) {
-    if (recent) return 0xffffffffu;
-    if (w != w) return 0xfffffffeu;
     const uint32_t u = __float_as_uint(w + 0.0f);  // (-0 becomes +0)
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const uint32_t key = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    return recent ? 0xffffffffu : w != w ? 0xfffffffeu : key;
 }
+template <int KEYS>  // rows a thread holds: up to KEYS * SELECT_TPB in all; 0: none, they are read every time
 __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t pick[2];
-    __shared__ int waves[2][SELECT_TPB / 64];
+    constexpr int WAVES = SELECT_TPB / 64;
+    __shared__ uint32_t hist[8][256];
+    __shared__ int waves[2][WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int i = blockIdx.x / a.p.heads, h = blockIdx.x - i * a.p.heads, len = a.len[i];
     int32_t *out = a.moves + (int64_t)blockIdx.x * (2 * (int64_t)a.cap + 1);
@@ -176,65 +187,92 @@ __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArg
     const int64_t at = ((int64_t)a.slot[i] * a.p.heads + h) * a.p.max_len;
     const float *w = a.p.weight + at;
     const int32_t *pos = a.p.pos + at;
-    const int recent_from = a.seen[i] - a.recent;
-    auto key_of = [&](int t) { return weight_key(w[t], pos[t] >= recent_from); };
-    // Of the values value(t) with ok(t): the `want`-th in descending order (want >= 1), and how many of its equals
-    // belong to the first `want`.
-    auto select = [&](auto ok, auto value, uint32_t want, uint32_t &found, uint32_t &equals) {
-        uint32_t prefix = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int j = tid; j < 256; j += SELECT_TPB) hist[j] = 0;
-            __syncthreads();
-            for (int t = tid; t < len; t += SELECT_TPB)
-                if (ok(t)) {
-                    const uint32_t v = value(t);
-                    if (shift == 24 || (v >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(v >> shift) & 255], 1u);
-                }
-            __syncthreads();
-            if (wave == 0) {  // lane: bins 255 - 4 lane down to 252 - 4 lane, descending
-                uint32_t c[4], mine = 0;
-                for (int j = 0; j < 4; ++j) { c[j] = hist[255 - 4 * lane - j]; mine += c[j]; }
-                uint32_t before = mine;
-                for (int off = 1; off < 64; off <<= 1) {
-                    const uint32_t x = __shfl_up(before, off, 64);
-                    if (lane >= off) before += x;
-                }
-                before -= mine;
-                for (int j = 0; j < 4; ++j) {
-                    if (before < want && want <= before + c[j]) {
-                        pick[0] = (uint32_t)(255 - 4 * lane - j);
-                        pick[1] = want - before;
-                    }
-                    before += c[j];
-                }
+    const int recent_from = a.seen[i] - a.recent, top = a.seen[i];  // positions are below `top`
+    for (int j = tid; j < 8 * 256; j += SELECT_TPB) hist[j >> 8][j & 255] = 0;
+    uint32_t held[KEYS ? KEYS : 1];
+    if (KEYS) {  // (all asked for before the first is looked at)
+        float hw[KEYS ? KEYS : 1];
+        int hp[KEYS ? KEYS : 1];
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j)
+            if (j * SELECT_TPB < len) {
+                const int t = min(tid + j * SELECT_TPB, len - 1);
+                hw[j] = w[t];
+                hp[j] = pos[t];
             }
-            __syncthreads();
-            prefix |= pick[0] << shift;
-            want = pick[1];
-            __syncthreads();
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j) held[j] = j * SELECT_TPB < len ? weight_key(hw[j], hp[j] >= recent_from) : 0;
+    }
+    __syncthreads();
+    // f(key, row) for every row this thread looks at; whole wavefronts call it together
+    auto each = [&](auto f) {
+        if (KEYS) {
+#pragma unroll
+            for (int j = 0; j < KEYS; ++j)
+                if (j * SELECT_TPB < len) f(held[j], tid + j * SELECT_TPB);
+        } else {
+            for (int base = 0; base < len; base += SELECT_TPB) {
+                const int t = base + tid;
+                f(weight_key(w[min(t, len - 1)], pos[min(t, len - 1)] >= recent_from), t);
+            }
         }
-        found = prefix;
-        equals = want;
     };
-    uint32_t key, ties;
-    select([&](int) { return true; }, key_of, (uint32_t)a.budget, key, ties);
-    // of the rows with that key the `ties` earliest stay: positions are below 2^31, so ~pos descends as they ascend
-    uint32_t last, unused;
-    select([&](int t) { return key_of(t) == key; }, [&](int t) { return ~(uint32_t)pos[t]; }, ties, last, unused);
-    int holes = 0, movers = 0;
-    for (int base = 0; base < len; base += SELECT_TPB) {
-        const int t = base + tid;
-        bool stays = false;
-        if (t < len) {
-            const uint32_t k = key_of(t);
-            stays = k > key || (k == key && ~(uint32_t)pos[t] >= last);
+    // Of the values value(key, row) of the rows with takes(key, row): the `want`-th in descending order.  `equals`: how many
+    // rows with that value are among the first `want`, `all`: how many there are.
+    int slot = 0;
+    auto search = [&](int digits, uint32_t want, auto takes, auto value, uint32_t &equals, uint32_t &all) {
+        uint32_t found = 0;
+#pragma unroll 1
+        for (int shift = 8 * (digits - 1); shift >= 0; shift -= 8, ++slot) {
+            each([&](uint32_t key, int t) {
+                const uint32_t v = value(key, t);
+                if (t < len && takes(key, t) && ((v ^ found) >> shift) < 256) atomicAdd(&hist[slot][(v >> shift) & 255], 1u);
+            });
+            __syncthreads();
+            // lane: digits 255 - 4 lane down to 252 - 4 lane
+            const uint4 h4 = *reinterpret_cast<const uint4 *>(&hist[slot][252 - 4 * lane]);
+            const uint32_t c[4] = {h4.w, h4.z, h4.y, h4.x};
+            uint32_t before = c[0] + c[1] + c[2] + c[3];
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const uint32_t x = __shfl_up(before, off, 64);
+                if (lane >= off) before += x;
+            }
+            const int at_lane = __ffsll((unsigned long long)__ballot(before >= want)) - 1;
+            before -= c[0] + c[1] + c[2] + c[3];
+            uint32_t digit = 0, rest = 0, count = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (before < want && want <= before + c[j]) {
+                    digit = (uint32_t)(255 - 4 * lane - j);
+                    rest = want - before;
+                    count = c[j];
+                }
+                before += c[j];
+            }
+            found |= (uint32_t)__builtin_amdgcn_readlane((int)digit, at_lane) << shift;
+            want = (uint32_t)__builtin_amdgcn_readlane((int)rest, at_lane);
+            all = (uint32_t)__builtin_amdgcn_readlane((int)count, at_lane);
         }
-        const bool hole = t < a.budget && !stays, mover = t >= a.budget && t < len && stays;
+        equals = want;
+        return found;
+    };
+    uint32_t ties, equal, late = 0, unused;
+    const uint32_t key = search(4, (uint32_t)a.budget, [](uint32_t, int) { return true; }, [](uint32_t k, int) { return k; }, ties, equal);
+    if (ties < equal) {  // of the rows with that key the earliest stay: those of a value top - 1 - position of at least `late`
+        const int digits = (39 - __clz(top > 1 ? top - 1 : 1)) / 8;
+        late = search(digits, ties, [&](uint32_t k, int) { return k == key; }, [&](uint32_t, int t) { return (uint32_t)(top - 1 - pos[min(t, len - 1)]); }, unused,
+                      unused);
+    }
+    int holes = 0, movers = 0;
+    each([&](uint32_t k, int t) {
+        const bool stays = t < len && (k > key || (k == key && (late == 0 || (uint32_t)(top - 1 - pos[min(t, len - 1)]) >= late)));
+        const bool hole = t < a.budget && !stays, mover = t >= a.budget && stays;
         const unsigned long long hb = __ballot(hole), mb = __ballot(mover), below = (1ull << lane) - 1;
         if (lane == 0) { waves[0][wave] = __popcll(hb); waves[1][wave] = __popcll(mb); }
         __syncthreads();
         int ho = holes, mo = movers;
-        for (int x = 0; x < SELECT_TPB / 64; ++x) {
+        for (int x = 0; x < WAVES; ++x) {
             if (x < wave) { ho += waves[0][x]; mo += waves[1][x]; }
             holes += waves[0][x];
             movers += waves[1][x];
@@ -242,10 +280,12 @@ __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArg
         if (hole && ho + __popcll(hb & below) < a.cap) out[1 + ho + __popcll(hb & below)] = t;
         if (mover && mo + __popcll(mb & below) < a.cap) out[1 + a.cap + mo + __popcll(mb & below)] = t;
         __syncthreads();
-    }
+    });
     if (tid == 0) out[0] = min(min(holes, movers), a.cap);
 }
-// A wavefront per move; blockIdx.y: (sequence, head).
+// A wavefront per move; blockIdx.y: (sequence, head).  Rows are stored past the caches (nontemporal): left in the last-level
+// cache they are written back under the next attention's reads (1.07 GB of rows behind 230 MB of moves and appends: 214 us
+// instead of 162; the moves themselves take 37 us either way).
 __global__ __launch_bounds__(TPB) void paged_move_kernel(const EvictArgs a) {
     const PagedPool &p = a.p;
     const int i = blockIdx.y / p.heads, h = blockIdx.y - i * p.heads, lane = threadIdx.x & 63;
@@ -258,9 +298,9 @@ __global__ __launch_bounds__(TPB) void paged_move_kernel(const EvictArgs a) {
     const int bytes = p.d * (p.quantized ? 1 : 4);
     if (bytes % 16 == 0) {
         for (int c = lane; c < bytes / 16; c += 64) {
-            const int4 k = reinterpret_cast<const int4 *>((const char *)p.k + src * bytes)[c], v = reinterpret_cast<const int4 *>((const char *)p.v + src * bytes)[c];
-            reinterpret_cast<int4 *>((char *)p.k + dst * bytes)[c] = k;
-            reinterpret_cast<int4 *>((char *)p.v + dst * bytes)[c] = v;
+            const i32x4 k = reinterpret_cast<const i32x4 *>((const char *)p.k + src * bytes)[c], v = reinterpret_cast<const i32x4 *>((const char *)p.v + src * bytes)[c];
+            __builtin_nontemporal_store(k, reinterpret_cast<i32x4 *>((char *)p.k + dst * bytes) + c);
+            __builtin_nontemporal_store(v, reinterpret_cast<i32x4 *>((char *)p.v + dst * bytes) + c);
         }
     } else {
         for (int c = lane; c < bytes; c += 64) {
@@ -281,6 +321,7 @@ void launch_append(const PagedPool &p, const PagedNew &in, const PagedAppend &a)
     const uint32_t rows = (uint32_t)a.n * p.heads * in.tokens;
     MNI_KERNEL_LAUNCH((paged_append_kernel<Q8, VEC, LPR>), dim3((rows + TPB / LPR - 1) / (TPB / LPR)), dim3(TPB), 0, ctx().stream, p, in, a);
 }
+
 }  // namespace
 
 int k_paged_table(const PagedPool &p, const PagedTableWrite &w) {
@@ -357,7 +398,10 @@ int k_paged_evict(const PagedPool &p, const PagedSeqs &s, const int32_t *seen, i
     void *moves = nullptr;
     MNI_TRY(dev_alloc(&moves, (size_t)s.n * p.heads * (2 * (size_t)a.cap + 1) * sizeof(int32_t)));
     a.moves = (int32_t *)moves;
-    MNI_KERNEL_LAUNCH(paged_select_kernel, dim3((unsigned)(s.n * p.heads)), dim3(SELECT_TPB), 0, ctx().stream, a);
+    const dim3 grid((unsigned)(s.n * p.heads));
+    if (longest <= 8 * SELECT_TPB) MNI_KERNEL_LAUNCH(paged_select_kernel<8>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
+    else if (longest <= 32 * SELECT_TPB) MNI_KERNEL_LAUNCH(paged_select_kernel<32>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
+    else MNI_KERNEL_LAUNCH(paged_select_kernel<0>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
     int rc = check_launch("paged_select");
     if (rc == MNI_OK) {
         MNI_KERNEL_LAUNCH(paged_move_kernel, dim3((unsigned)((a.cap + 3) / 4), (unsigned)(s.n * p.heads)), dim3(TPB), 0, ctx().stream, a);

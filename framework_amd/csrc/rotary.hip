@@ -2,6 +2,7 @@
 // (mni_rocm_qk_norm_rope).  Bandwidth-bound: 8 bytes an element forward (one read, one write), 12 backward; what the
 // chip could waste on top are the sines, so a group of lanes keeps its token's and uses them for several heads.
 #include <math.h>
+#include <string.h>
 
 #include "common.h"
 #include "lanes.h"
@@ -196,6 +197,7 @@ __global__ __launch_bounds__(1024) void rope_dgamma_kernel(const RopeArgs a, int
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dim = blockIdx.x * 64 + lane;
     float sum = 0.f;
     if (dim < a.d)
+#pragma unroll 8
         for (int r = wave; r < rows; r += 16) sum += a.part[((int64_t)blockIdx.y * rows + r) * a.d + dim];
     red[wave][lane] = sum;
     __syncthreads();
@@ -333,8 +335,15 @@ int rope_args(const mni_rope_desc &d, bool backward, RopeArgs *a) {
     a->chunks = 1;
     a->eps = (float)d.eps;
     a->inv_d = 1.0f / (float)d.head_dim;
-    for (int i = 0; i < ROPE_MAX_DIM / 2; ++i)
-        a->turns[i] = i < a->rot / 2 ? pow(d.theta, -2.0 * i / a->rot) / (2.0 * M_PI) : 0.0;
+    // The last plan's frequencies are kept (a model has one): 64 powers cost as long as a launch.
+    static double turns[ROPE_MAX_DIM / 2], of_theta = 0.0;
+    static int of_rot = -1;
+    if (of_theta != d.theta || of_rot != a->rot) {
+        for (int i = 0; i < ROPE_MAX_DIM / 2; ++i) turns[i] = i < a->rot / 2 ? pow(d.theta, -2.0 * i / a->rot) / (2.0 * M_PI) : 0.0;
+        of_theta = d.theta;
+        of_rot = a->rot;
+    }
+    memcpy(a->turns, turns, sizeof turns);
     return MNI_OK;
 }
 template <int LPR>

@@ -14,6 +14,8 @@ importing a symbol from it raises.
 """
 import ctypes as C
 import os
+import struct
+from array import array
 
 import numpy as np
 
@@ -59,6 +61,9 @@ class RopeDesc(C.Structure):
                 ("q", RopeHeads), ("k", RopeHeads)]
 
 
+_ROPE_DESC = struct.Struct("<4qQ2q2d2i" + "Q4q5Q" * 2)  # RopeDesc: packing one is several times quicker than filling its fields
+
+
 # name -> (restype, argtypes): every symbol include/mni_rocm.h declares.
 SIGNATURES = {
     "mni_rocm_init": (C.c_int, [C.c_int]),
@@ -95,8 +100,8 @@ SIGNATURES = {
     "mni_rocm_unbroadcast": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_int64), C.c_int, C.POINTER(C.c_int64), C.c_int]),
     "mni_rocm_axpy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_float, C.c_int64]),
     "mni_rocm_fill": (C.c_int, [C.c_void_p, C.c_float, C.c_int64]),
-    "mni_rocm_qk_norm_rope": (C.c_int, [C.POINTER(RopeDesc)]),
-    "mni_rocm_qk_norm_rope_backward": (C.c_int, [C.POINTER(RopeDesc)]),
+    "mni_rocm_qk_norm_rope": (C.c_int, [C.c_void_p]),  # a RopeDesc, packed
+    "mni_rocm_qk_norm_rope_backward": (C.c_int, [C.c_void_p]),
     "mni_zeros": (C.c_uint32, [_i64p, C.c_int]),
     "mni_ones": (C.c_uint32, [_i64p, C.c_int]),
     "mni_from_float32": (C.c_uint32, [C.c_void_p, C.c_size_t, _i64p, C.c_int]),
@@ -170,12 +175,12 @@ SIGNATURES = {
     "mni_paged_cache_add": (C.c_uint32, [C.c_uint32]), "mni_paged_cache_fork": (C.c_uint32, [C.c_uint32] * 2),
     "mni_paged_cache_drop": (C.c_int, [C.c_uint32] * 2),
     "mni_paged_cache_len": (C.c_int64, [C.c_uint32] * 2), "mni_paged_cache_seen": (C.c_int64, [C.c_uint32] * 2),
-    "mni_paged_cache_append": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, C.c_uint32, C.c_uint32, _i64p]),
-    "mni_paged_cache_truncate": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, _i64p]),
-    "mni_paged_cache_attend": (C.c_uint32, [C.c_uint32, _u32p, C.c_size_t, C.c_uint32, C.c_double, C.c_int]),
-    "mni_paged_cache_add_weights": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, C.c_uint32]),
-    "mni_paged_cache_evict": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, C.c_int64, C.c_int64]),
-    "mni_paged_cache_track": (C.c_int, [C.c_uint32, _u32p, C.c_size_t, _u32p, _u32p]),
+    "mni_paged_cache_append": (C.c_int, [C.c_uint32, C.c_void_p, C.c_size_t, C.c_uint32, C.c_uint32, C.c_void_p]),
+    "mni_paged_cache_truncate": (C.c_int, [C.c_uint32, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mni_paged_cache_attend": (C.c_uint32, [C.c_uint32, C.c_void_p, C.c_size_t, C.c_uint32, C.c_double, C.c_int]),
+    "mni_paged_cache_add_weights": (C.c_int, [C.c_uint32, C.c_void_p, C.c_size_t, C.c_uint32]),
+    "mni_paged_cache_evict": (C.c_int, [C.c_uint32, C.c_void_p, C.c_size_t, C.c_int64, C.c_int64]),
+    "mni_paged_cache_track": (C.c_int, [C.c_uint32, C.c_void_p, C.c_size_t, _u32p, _u32p]),
     "mni_paged_cache_read": (C.c_int, [C.c_uint32, C.c_uint32, _u32p]),
     "mni_dev_ptr": (C.c_void_p, [C.c_uint32]),
     "mni_rocm_int_buffer_ptr": (C.c_void_p, [C.c_uint32]),
@@ -207,6 +212,14 @@ def _i64_array(values):
 
 def _u32_array(values):
     return (C.c_uint32 * max(len(values), 1))(*[int(v) for v in values])
+
+
+def _packed(kind, values):
+    """A list of ids ("I") or of int64 ("q") as the bytes of a C array."""
+    try:
+        return array(kind, values).tobytes()
+    except OverflowError as e:
+        raise MniError("id or length out of range: %s" % e)
 
 
 class Rocm:
@@ -382,24 +395,32 @@ class Rocm:
         self._check(self.lib.mni_rocm_fill(dst, value, n))
 
     @staticmethod
-    def rope_desc(q, k=None, *, batch, seq, head_dim, rotary_dims=None, positions=None, position_stride=0, offset=0, interleaved=False,
-                  theta=10000.0, eps=1e-6):
-        """q, k: dicts of device addresses x, gamma and out (forward) or grad, dx and dgamma (backward), `heads`, and
-        `strides` of x in elements (batch, head, token; default: x contiguous [batch, heads, seq, head_dim])."""
+    def _rope_packed(q, k=None, *, batch, seq, head_dim, rotary_dims=None, positions=None, position_stride=0, offset=0, interleaved=False,
+                     theta=10000.0, eps=1e-6):
         def heads(o):
             if o is None:
-                return RopeHeads()
-            s = o.get("strides") or (o["heads"] * seq * head_dim, seq * head_dim, head_dim)
-            return RopeHeads(o["x"], o["heads"], s[0], s[1], s[2], o["gamma"], o.get("out"), o.get("grad"), o.get("dx"), o.get("dgamma"))
-        return RopeDesc(batch, seq, head_dim, head_dim if rotary_dims is None else rotary_dims, positions, position_stride, offset, theta, eps,
-                        1 if interleaved else 0, 0, heads(q), heads(k))
+                return (0,) * 10
+            get = o.get
+            b, h, s = get("strides") or (o["heads"] * seq * head_dim, seq * head_dim, head_dim)
+            return (o["x"] or 0, o["heads"], b, h, s, o["gamma"] or 0, get("out") or 0, get("grad") or 0, get("dx") or 0, get("dgamma") or 0)
+        return _ROPE_DESC.pack(batch, seq, head_dim, head_dim if rotary_dims is None else rotary_dims, positions or 0, position_stride, offset,
+                               theta, eps, 1 if interleaved else 0, 0, *heads(q), *heads(k))
+
+    @classmethod
+    def rope_desc(cls, q, k=None, **plan):
+        """q, k: dicts of device addresses x, gamma and out (forward) or grad, dx and dgamma (backward), `heads`, and
+        `strides` of x in elements (batch, head, token; default: x contiguous [batch, heads, seq, head_dim]).  plan: batch,
+        seq, head_dim, rotary_dims (all), positions (an address; 0 .. seq - 1), position_stride, offset, interleaved, theta, eps."""
+        return RopeDesc.from_buffer_copy(cls._rope_packed(q, k, **plan))
 
     def qk_norm_rope(self, q, k=None, **plan):
         """Norm of queries and keys for each head and the rotation of their positions, in one launch (see rope_desc)."""
-        self._check(self.lib.mni_rocm_qk_norm_rope(C.byref(self.rope_desc(q, k, **plan))))
+        if self.lib.mni_rocm_qk_norm_rope(self._rope_packed(q, k, **plan)):
+            self._check(1)
 
     def qk_norm_rope_backward(self, q, k=None, **plan):
-        self._check(self.lib.mni_rocm_qk_norm_rope_backward(C.byref(self.rope_desc(q, k, **plan))))
+        if self.lib.mni_rocm_qk_norm_rope_backward(self._rope_packed(q, k, **plan)):
+            self._check(1)
 
 
 class Native:
@@ -600,25 +621,25 @@ class Native:
     def pagedCacheAppend(self, cacheId, seqs, k, v, counts=None):
         if counts is not None and len(counts) != len(seqs):
             raise MniError("paged cache append: %d counts for %d sequences" % (len(counts), len(seqs)))
-        self._rc(self.lib.mni_paged_cache_append(cacheId, _u32_array(seqs), len(seqs), k, v, None if counts is None else _i64_array(counts)))
+        self._rc(self.lib.mni_paged_cache_append(cacheId, _packed("I", seqs), len(seqs), k, v, None if counts is None else _packed("q", counts)))
 
     def pagedCacheTruncate(self, cacheId, seqs, lens):
         if len(lens) != len(seqs):
             raise MniError("paged cache truncate: %d lengths for %d sequences" % (len(lens), len(seqs)))
-        self._rc(self.lib.mni_paged_cache_truncate(cacheId, _u32_array(seqs), len(seqs), _i64_array(lens)))
+        self._rc(self.lib.mni_paged_cache_truncate(cacheId, _packed("I", seqs), len(seqs), _packed("q", lens)))
 
     def pagedCacheAttend(self, cacheId, seqs, q, scale, accumulate):
-        return self._id(self.lib.mni_paged_cache_attend(cacheId, _u32_array(seqs), len(seqs), q, scale, 1 if accumulate else 0))
+        return self._id(self.lib.mni_paged_cache_attend(cacheId, _packed("I", seqs), len(seqs), q, scale, 1 if accumulate else 0))
 
     def pagedCacheAddWeights(self, cacheId, seqs, w):
-        self._rc(self.lib.mni_paged_cache_add_weights(cacheId, _u32_array(seqs), len(seqs), w))
+        self._rc(self.lib.mni_paged_cache_add_weights(cacheId, _packed("I", seqs), len(seqs), w))
 
     def pagedCacheEvict(self, cacheId, seqs, budget, recent):
-        self._rc(self.lib.mni_paged_cache_evict(cacheId, _u32_array(seqs), len(seqs), budget, recent))
+        self._rc(self.lib.mni_paged_cache_evict(cacheId, _packed("I", seqs), len(seqs), budget, recent))
 
     def pagedCacheTrack(self, cacheId, seqs):
         w, p = C.c_uint32(0), C.c_uint32(0)
-        self._rc(self.lib.mni_paged_cache_track(cacheId, _u32_array(seqs), len(seqs), C.byref(w), C.byref(p)))
+        self._rc(self.lib.mni_paged_cache_track(cacheId, _packed("I", seqs), len(seqs), C.byref(w), C.byref(p)))
         return [w.value, p.value]
 
     def pagedCacheRead(self, cacheId, seq):

@@ -258,7 +258,8 @@ def test_random_program(gpu, seed, heads, group, d, page, quantized):
     assert cache.freePages() == pages
 
 
-@pytest.mark.parametrize("length,budget,recent", [(65, 64, 0), (5000, 500, 100), (300, 299, 299), (1100, 1024, 7), (2048, 1, 0), (2048, 1, 1), (700, 650, 0), (40, 0, 0)])
+@pytest.mark.parametrize("length,budget,recent", [(65, 64, 0), (5000, 500, 100), (300, 299, 299), (1100, 1024, 7), (2048, 1, 0), (2048, 1, 1), (700, 650, 0), (40, 0, 0),
+                                                  (9000, 8100, 1000), (33000, 3000, 50)])
 @pytest.mark.parametrize("kind", ["spread", "equal", "extremes"])
 def test_eviction_keeps_the_heaviest(gpu, length, budget, recent, kind):
     heads, d, page = 2, 16, 16

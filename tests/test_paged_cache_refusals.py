@@ -62,3 +62,8 @@ def test_binding_layout():
     # mni_rope_heads: pointer, 4 x int64, 5 pointers; mni_rope_desc as laid out in the header
     assert ctypes.sizeof(N.RopeHeads) == 80 and N.RopeHeads.gamma.offset == 40
     assert ctypes.sizeof(N.RopeDesc) == 9 * 8 + 8 + 160 and N.RopeDesc.q.offset == 80
+    d = N.Rocm.rope_desc(dict(x=5, heads=2, strides=(9, 8, 7), gamma=6, out=4), dict(x=1, heads=3, gamma=2, dgamma=11), batch=2, seq=3, head_dim=8, rotary_dims=4,
+                         positions=13, position_stride=3, offset=-1, interleaved=True, theta=2.0, eps=0.5)
+    assert (d.batch, d.seq, d.head_dim, d.rotary_dims, d.positions, d.position_stride, d.offset, d.theta, d.eps, d.interleaved) == (2, 3, 8, 4, 13, 3, -1, 2.0, 0.5, 1)
+    assert (d.q.x, d.q.heads, d.q.batch_stride, d.q.head_stride, d.q.token_stride, d.q.gamma, d.q.out, d.q.grad) == (5, 2, 9, 8, 7, 6, 4, None)
+    assert (d.k.x, d.k.batch_stride, d.k.head_stride, d.k.token_stride, d.k.dgamma) == (1, 72, 24, 8, 11)
