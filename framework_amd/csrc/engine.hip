@@ -1947,7 +1947,7 @@ static int paged_unshare(PagedCache &c, uint32_t seq, int64_t from, int64_t to, 
     for (int64_t j = from; j < to; ++j) {
         const int32_t page = s.pages[j];
         if (c.holders[page] <= 1) continue;
-        if (copies.n == PAGED_PAIRS / 2) {
+        if (copies.n == PAGED_COPIES) {
             MNI_TRY(k_paged_copy(c.pool, copies));
             copies.n = 0;
         }
@@ -2042,32 +2042,12 @@ static uint32_t paged_fork(PagedCache &c, uint32_t from) {
     for (int32_t page : c.seqs[seq].pages) ++c.holders[page];
     return seq;
 }
-// New table entries: up to a few hundred travel in a launch's arguments, more go up as the runs that they are.
-static int paged_write_table(PagedCache &c, const uint32_t *seqs, const std::vector<int64_t> &had, size_t total) {
-    if (total == 0) return MNI_OK;
-    if (total > 4 * PAGED_PAIRS / 2) {
-        for (size_t i = 0; i < had.size(); ++i) {
-            const std::vector<int32_t> &pages = c.seqs[seqs[i]].pages;
-            for (size_t j = (size_t)had[i]; j < pages.size(); j += DeviceCtx::STAGE_BYTES / 4)
-                MNI_TRY(upload_small(c.pool.table + paged_entry(c, seqs[i], (int64_t)j), pages.data() + j,
-                                     std::min<size_t>(DeviceCtx::STAGE_BYTES / 4, pages.size() - j) * 4));
-        }
-        return MNI_OK;
-    }
-    PagedTableWrite w;
-    w.n = 0;
-    for (size_t i = 0; i < had.size(); ++i) {
-        const std::vector<int32_t> &pages = c.seqs[seqs[i]].pages;
-        for (size_t j = (size_t)had[i]; j < pages.size(); ++j) {
-            w.at[w.n] = paged_entry(c, seqs[i], (int64_t)j);
-            w.page[w.n++] = pages[j];
-            if (w.n == PAGED_PAIRS / 2) {
-                MNI_TRY(k_paged_table(c.pool, w));
-                w.n = 0;
-            }
-        }
-    }
-    return k_paged_table(c.pool, w);
+// Entries of the table for more new pages than a launch's arguments hold: they go up as the run that they are.
+static int paged_write_table(PagedCache &c, uint32_t seq, int64_t had) {
+    const std::vector<int32_t> &pages = c.seqs[seq].pages;
+    for (size_t j = (size_t)had; j < pages.size(); j += DeviceCtx::STAGE_BYTES / 4)
+        MNI_TRY(upload_small(c.pool.table + paged_entry(c, seq, (int64_t)j), pages.data() + j, std::min<size_t>(DeviceCtx::STAGE_BYTES / 4, pages.size() - j) * 4));
+    return MNI_OK;
 }
 static int paged_append(PagedCache &c, const uint32_t *seqs, size_t n, uint32_t k, uint32_t v, const int64_t *counts) {
     MNI_TRY(paged_check(c, seqs, n, true, "append"));
@@ -2120,31 +2100,63 @@ static int paged_append(PagedCache &c, const uint32_t *seqs, size_t n, uint32_t 
     PagedCopies copies;
     copies.n = 0;
     std::vector<int64_t> had(n);
-    size_t total = 0;
     for (size_t i = 0; i < n; ++i) {
         PagedSequence &s = c.seqs[seqs[i]];
         const int64_t count = counts ? counts[i] : tokens;
         if (count > 0 && (s.len & (p.page - 1))) MNI_TRY(paged_unshare(c, seqs[i], (int64_t)s.pages.size() - 1, (int64_t)s.pages.size(), copies));
         had[i] = (int64_t)s.pages.size();
-        while ((int64_t)s.pages.size() < paged_pages(c, s.len + count)) { s.pages.push_back(paged_take(c)); ++total; }
+        while ((int64_t)s.pages.size() < paged_pages(c, s.len + count)) s.pages.push_back(paged_take(c));
     }
     MNI_TRY(k_paged_copy(p, copies));
-    if (tokens > 1) MNI_TRY(paged_write_table(c, seqs, had, total));
-    for (size_t first = 0; first < n; first += PAGED_BATCH) {
-        PagedAppend a;
-        a.n = (int)std::min<size_t>(PAGED_BATCH, n - first);
-        for (int i = 0; i < a.n; ++i) {
-            PagedSequence &s = c.seqs[seqs[first + i]];
-            a.slot[i] = (int32_t)seqs[first + i];
-            a.len[i] = (int32_t)s.len;
-            a.count[i] = (int32_t)(counts ? counts[first + i] : tokens);
-            a.seen[i] = (int32_t)s.seen;
-            a.page[i] = tokens == 1 && (int64_t)s.pages.size() > had[first + i] ? s.pages.back() : -1;
-            s.len += a.count[i];
-            s.seen += a.count[i];
-        }
+    auto inputs = [&](size_t first) {
         in.k = kb->p + (int64_t)first * in.k_seq;
         in.v = vb->p + (int64_t)first * in.v_seq;
+    };
+    auto enter = [&](auto &a, size_t i) {
+        PagedSequence &s = c.seqs[seqs[i]];
+        const int k = a.n++;
+        a.slot[k] = (int32_t)seqs[i];
+        a.len[k] = (int32_t)s.len;
+        a.count[k] = (int32_t)(counts ? counts[i] : tokens);
+        a.seen[k] = (int32_t)s.seen;
+        s.len += a.count[k];
+        s.seen += a.count[k];
+        return k;
+    };
+    if (tokens == 1) {
+        for (size_t first = 0; first < n; first += PagedAppend::MAX) {
+            PagedAppend a;
+            a.n = 0;
+            inputs(first);
+            for (size_t i = first; i < n && a.n < PagedAppend::MAX; ++i) {
+                const int k = enter(a, i);
+                const PagedSequence &s = c.seqs[seqs[i]];
+                a.page[k] = (int64_t)s.pages.size() > had[i] ? s.pages.back() : -1;
+            }
+            MNI_TRY(k_paged_append(p, in, a));
+        }
+        return MNI_OK;
+    }
+    for (size_t first = 0; first < n;) {
+        PagedPrompt a;
+        a.n = 0;
+        inputs(first);
+        int used = 0;
+        for (; first < n && a.n < PagedPrompt::MAX; ++first) {
+            const std::vector<int32_t> &pages = c.seqs[seqs[first]].pages;
+            const int64_t fresh = (int64_t)pages.size() - had[first];
+            if (fresh <= PAGED_PROMPT_PAGES && used + fresh > PAGED_PROMPT_PAGES) break;  // (fits the next launch's)
+            const int k = enter(a, first);
+            a.first[k] = used;
+            a.had[k] = (int32_t)had[first];
+            if (fresh > PAGED_PROMPT_PAGES) {
+                MNI_TRY(paged_write_table(c, seqs[first], had[first]));
+                a.had[k] = INT32_MAX;
+            } else {
+                std::copy(pages.begin() + had[first], pages.end(), a.pages + used);
+                used += (int)fresh;
+            }
+        }
         MNI_TRY(k_paged_append(p, in, a));
     }
     return MNI_OK;

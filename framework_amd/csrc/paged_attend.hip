@@ -350,8 +350,8 @@ __device__ __forceinline__ TileWork tile_work(const AttendArgs &a, int32_t *stag
     return w;
 }
 // accumulate: a chunk's scores are kept in LDS, [head][positions + 4] (the odd 16 bytes spread a wavefront's four quarters
-// over the banks), and leave at the end in whole lines.  Written tile by tile, 64 bytes a head, they cost 34 us on 131072
-// positions of 32 heads (17 MB among 1.1 GB of reads), of which the lines' halves coming apart were two thirds.
+// over the banks), and leave at the end in whole lines, past the caches.  On 131072 positions of 32 heads (17 MB among 1.1
+// GB of reads) they cost 14 us so, 20 through the caches, and 34 written tile by tile, 64 bytes a head.
 template <int T>
 __device__ __forceinline__ void tile_scores_keep(float *scores, const TileWork &w, const f32x4 (&s)[T], int base, int lane) {
     if ((lane & 15) >= w.heads) return;
@@ -367,7 +367,7 @@ __device__ __forceinline__ void tile_scores_out(const AttendArgs &a, const TileW
     for (int g = 0; g < w.heads; ++g) {
         float *out = scores_of(a, w.i, w.head0 + g) + w.t0;  // (a head's row begins on a multiple of four and is as long as one)
         for (int at = 4 * (int)threadIdx.x; at < w.n; at += 4 * TPB)
-            *reinterpret_cast<f32x4 *>(out + at) = *reinterpret_cast<const f32x4 *>(scores + g * (w.chunk + 4) + at);
+            __builtin_nontemporal_store(*reinterpret_cast<const f32x4 *>(scores + g * (w.chunk + 4) + at), reinterpret_cast<f32x4 *>(out + at));
     }
 }
 

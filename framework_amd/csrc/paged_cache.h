@@ -28,21 +28,27 @@ struct PagedNew {
     int64_t k_seq, k_head, k_token, v_seq, v_head, v_token;
     int tokens;  // rows per (sequence, head) in the input; counts[i] of them are taken
 };
+// The sequences of an append and the pages that their new rows go to.  PagedAppend: one token each; page[i] is its new
+// page, or -1 (the table has it).  PagedPrompt: several; pages from had[i] on are pages[first[i] ..] (had[i] = INT32_MAX:
+// the table has them all).  The kernel enters the new ones into the table.
 struct PagedAppend {
+    static constexpr int MAX = PAGED_BATCH;
     int n;
-    int32_t slot[PAGED_BATCH], len[PAGED_BATCH], count[PAGED_BATCH], seen[PAGED_BATCH];
-    int32_t page[PAGED_BATCH];  // tokens == 1: the new page of this token, or -1 (the table has it)
+    int32_t slot[MAX], len[MAX], count[MAX], seen[MAX];
+    int32_t page[MAX];
 };
-constexpr int PAGED_PAIRS = 448;  // entries of a table write or page copies in one launch's arguments
-struct PagedTableWrite {
+constexpr int PAGED_PROMPT_PAGES = 704;
+struct PagedPrompt {
+    static constexpr int MAX = 32;
     int n;
-    int64_t at[PAGED_PAIRS / 2];
-    int32_t page[PAGED_PAIRS / 2];
+    int32_t slot[MAX], len[MAX], count[MAX], seen[MAX], had[MAX], first[MAX];
+    int32_t pages[PAGED_PROMPT_PAGES];
 };
+constexpr int PAGED_COPIES = 224;  // page copies of one launch
 struct PagedCopies {
     int n;
-    int64_t at[PAGED_PAIRS / 2];  // table entry that gets the new page
-    int32_t from[PAGED_PAIRS / 2], to[PAGED_PAIRS / 2];
+    int64_t at[PAGED_COPIES];  // table entry that gets the new page
+    int32_t from[PAGED_COPIES], to[PAGED_COPIES];
 };
 
 #ifdef __HIPCC__
@@ -51,9 +57,9 @@ __device__ __forceinline__ int64_t row_of(const PagedPool &p, int page, int head
 }
 #endif
 
-int k_paged_table(const PagedPool &p, const PagedTableWrite &w);
 int k_paged_copy(const PagedPool &p, const PagedCopies &c);
 int k_paged_append(const PagedPool &p, const PagedNew &in, const PagedAppend &a);
+int k_paged_append(const PagedPool &p, const PagedNew &in, const PagedPrompt &a);
 // q, out: [n, q_heads, d], contiguous
 int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float *out, int q_heads, float scale, bool accumulate);
 // w: [n, heads, width], contiguous

@@ -9,10 +9,7 @@ namespace {
 constexpr int TPB = 256;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// ---- table entries, page copies, forks -----------------------------------------------------------------------------
-__global__ __launch_bounds__(TPB) void paged_table_kernel(int32_t *__restrict__ table, const PagedTableWrite w) {
-    for (int i = threadIdx.x; i < w.n; i += TPB) table[w.at[i]] = w.page[i];
-}
+// ---- page copies, forks -----------------------------------------------------------------------------
 // blockIdx.x: the copy, blockIdx.y: keys, values, key scales, value scales.  A page is one contiguous block.
 __global__ __launch_bounds__(TPB) void paged_copy_kernel(const PagedPool p, const PagedCopies c) {
     const int what = blockIdx.y;
@@ -52,8 +49,8 @@ struct AppendRow {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (VEC) {
-                if (4 * l < d) x[j] = *reinterpret_cast<const float4 *>(src + 4 * l);
+            if (VEC) {  // (the lanes behind the row repeat its last piece: no branch before the loads)
+                x[j] = *reinterpret_cast<const float4 *>(src + min(4 * l, d - 4));
             } else if (l + 64 * j < d) {
                 x[j].x = src[l + 64 * j];
             }
@@ -93,32 +90,41 @@ struct AppendRow {
         if (l == 0) scales[row] = scale;
     }
 };
-template <bool Q8, bool VEC, int LPR>
-__device__ __forceinline__ void append_store(const PagedPool &p, const PagedAppend &a, const AppendRow<VEC> &k, const AppendRow<VEC> &v, int page, int i, int h,
-                                             int t, int l) {
-    const int64_t at = (int64_t)a.len[i] + t, row = row_of(p, page, h, (int)(at & (p.page - 1)));
-    k.template store<Q8, LPR>(p.k, p.kscale, row, p.d, l);
-    v.template store<Q8, LPR>(p.v, p.vscale, row, p.d, l);
-    if (l == 0 && p.weight) {
-        const int64_t track = ((int64_t)a.slot[i] * p.heads + h) * p.max_len + at;
-        p.weight[track] = 0.f;
-        p.pos[track] = a.seen[i] + t;
-    }
+// The page of position `at` of sequence i, and whether it is a new one.
+__device__ __forceinline__ int page_of(const PagedPool &p, const PagedAppend &a, int i, int64_t at, bool &fresh) {
+    fresh = a.page[i] >= 0;
+    return fresh ? a.page[i] : p.table[a.slot[i] * p.max_pages + (at >> p.shift)];
 }
-// (Four rows a group, for prompts, measured no better: fp32 43.5 against 45 us on 134 MB, int8 14.3 against 11.3 on 29 MB.)
-template <bool Q8, bool VEC, int LPR>
-__global__ __launch_bounds__(TPB) void paged_append_kernel(const PagedPool p, const PagedNew in, const PagedAppend a) {
+__device__ __forceinline__ int page_of(const PagedPool &p, const PagedPrompt &a, int i, int64_t at, bool &fresh) {
+    const int index = (int)(at >> p.shift);
+    fresh = index >= a.had[i];
+    return fresh ? a.pages[a.first[i] + index - a.had[i]] : p.table[a.slot[i] * p.max_pages + index];
+}
+// A row of keys and values per group of LPR lanes.  (Four rows a group, all asked for before the first is stored: 68
+// against 46 us on 134 MB of fp32 rows, 13 against 10 on 29 MB of them stored as int8.)
+template <bool Q8, bool VEC, int LPR, class Batch>
+__global__ __launch_bounds__(TPB) void paged_append_kernel(const PagedPool p, const PagedNew in, const Batch a) {
     const uint32_t idx = blockIdx.x * (TPB / LPR) + threadIdx.x / LPR;
     const uint32_t ih = idx / (uint32_t)in.tokens, t = idx - ih * in.tokens;
     const uint32_t i = ih / (uint32_t)p.heads, h = ih - i * p.heads;
     if (i >= (uint32_t)a.n || t >= (uint32_t)a.count[i]) return;  // (whole groups leave)
-    const int l = threadIdx.x % LPR, fresh = a.page[i];
-    int32_t *entry = p.table + a.slot[i] * p.max_pages + (((int64_t)a.len[i] + t) >> p.shift);
+    const int l = threadIdx.x % LPR;
     AppendRow<VEC> k, v;
     k.load(in.k + i * in.k_seq + h * in.k_head + t * in.k_token, p.d, l);
     v.load(in.v + i * in.v_seq + h * in.v_head + t * in.v_token, p.d, l);
-    append_store<Q8, VEC, LPR>(p, a, k, v, fresh >= 0 ? fresh : *entry, i, h, t, l);
-    if (fresh >= 0 && h == 0 && l == 0) *entry = fresh;
+    const int64_t at = (int64_t)a.len[i] + t;
+    bool fresh;
+    const int page = page_of(p, a, (int)i, at, fresh), off = (int)(at & (p.page - 1));
+    const int64_t row = row_of(p, page, h, off);
+    k.template store<Q8, LPR>(p.k, p.kscale, row, p.d, l);
+    v.template store<Q8, LPR>(p.v, p.vscale, row, p.d, l);
+    if (l != 0) return;
+    if (fresh && h == 0 && off == 0) p.table[a.slot[i] * p.max_pages + (at >> p.shift)] = page;
+    if (p.weight) {
+        const int64_t track = ((int64_t)a.slot[i] * p.heads + h) * p.max_len + at;
+        p.weight[track] = 0.f;
+        p.pos[track] = a.seen[i] + t;
+    }
 }
 
 // ---- weights and positions -----------------------------------------------------------------------------------------
@@ -316,31 +322,13 @@ __global__ __launch_bounds__(TPB) void paged_move_kernel(const EvictArgs a) {
     }
 }
 
-template <bool Q8, bool VEC, int LPR>
-void launch_append(const PagedPool &p, const PagedNew &in, const PagedAppend &a) {
+template <bool Q8, bool VEC, int LPR, class Batch>
+void launch_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
     const uint32_t rows = (uint32_t)a.n * p.heads * in.tokens;
-    MNI_KERNEL_LAUNCH((paged_append_kernel<Q8, VEC, LPR>), dim3((rows + TPB / LPR - 1) / (TPB / LPR)), dim3(TPB), 0, ctx().stream, p, in, a);
+    MNI_KERNEL_LAUNCH((paged_append_kernel<Q8, VEC, LPR, Batch>), dim3((rows + TPB / LPR - 1) / (TPB / LPR)), dim3(TPB), 0, ctx().stream, p, in, a);
 }
-
-}  // namespace
-
-int k_paged_table(const PagedPool &p, const PagedTableWrite &w) {
-    if (w.n <= 0) return MNI_OK;
-    MNI_KERNEL_LAUNCH(paged_table_kernel, dim3(1), dim3(TPB), 0, ctx().stream, p.table, w);
-    return check_launch("paged_table");
-}
-int k_paged_copy(const PagedPool &p, const PagedCopies &c) {
-    if (c.n <= 0) return MNI_OK;
-    MNI_KERNEL_LAUNCH(paged_copy_kernel, dim3((unsigned)c.n, p.quantized ? 4 : 2), dim3(TPB), 0, ctx().stream, p, c);
-    return check_launch("paged_copy");
-}
-int k_paged_fork(const PagedPool &p, int32_t from, int32_t to, int64_t len) {
-    if (len <= 0) return MNI_OK;
-    const int heads = p.weight ? p.heads : 1;
-    MNI_KERNEL_LAUNCH(paged_fork_kernel, dim3((unsigned)((len + TPB - 1) / TPB), (unsigned)heads), dim3(TPB), 0, ctx().stream, p, from, to, len);
-    return check_launch("paged_fork");
-}
-int k_paged_append(const PagedPool &p, const PagedNew &in, const PagedAppend &a) {
+template <class Batch>
+int paged_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
     if (a.n <= 0 || in.tokens <= 0) return MNI_OK;
     const bool vec = p.d % 4 == 0 && (((uintptr_t)in.k | (uintptr_t)in.v) & 15) == 0 &&
                      ((in.k_seq | in.k_head | in.k_token | in.v_seq | in.v_head | in.v_token) & 3) == 0;
@@ -358,6 +346,22 @@ int k_paged_append(const PagedPool &p, const PagedNew &in, const PagedAppend &a)
     }
     return check_launch("paged_append");
 }
+
+}  // namespace
+
+int k_paged_copy(const PagedPool &p, const PagedCopies &c) {
+    if (c.n <= 0) return MNI_OK;
+    MNI_KERNEL_LAUNCH(paged_copy_kernel, dim3((unsigned)c.n, p.quantized ? 4 : 2), dim3(TPB), 0, ctx().stream, p, c);
+    return check_launch("paged_copy");
+}
+int k_paged_fork(const PagedPool &p, int32_t from, int32_t to, int64_t len) {
+    if (len <= 0) return MNI_OK;
+    const int heads = p.weight ? p.heads : 1;
+    MNI_KERNEL_LAUNCH(paged_fork_kernel, dim3((unsigned)((len + TPB - 1) / TPB), (unsigned)heads), dim3(TPB), 0, ctx().stream, p, from, to, len);
+    return check_launch("paged_fork");
+}
+int k_paged_append(const PagedPool &p, const PagedNew &in, const PagedAppend &a) { return paged_append(p, in, a); }
+int k_paged_append(const PagedPool &p, const PagedNew &in, const PagedPrompt &a) { return paged_append(p, in, a); }
 
 int k_paged_add_weights(const PagedPool &p, const PagedSeqs &s, const float *w, int64_t width) {
     int64_t longest = 0;
