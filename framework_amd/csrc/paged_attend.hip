@@ -30,18 +30,17 @@ struct AttendArgs {
     float *out;
     float *part;    // [chunk of the launch][q_heads][d]: sums not yet divided (null: every sequence is one chunk)
     float2 *ml;     // [chunk of the launch][q_heads]: maximum and sum
-    float2 *stats;  // accumulate: [sequence][q_heads], maximum and one over the sum
     float *scores;  // accumulate: see scores_of
     int n, q_heads, group, tiles_per_group, per_tile;
     int staged;  // words of LDS that page ids take before the scores that are kept there
     float scale;  // times log2 e
     int32_t slot[PAGED_BATCH], len[PAGED_BATCH], chunk[PAGED_BATCH];
     int32_t first[PAGED_BATCH + 1];          // first chunk of a sequence; INT_MAX behind the last sequence
-    int32_t tokens_before[PAGED_BATCH];  // of the sequences before, each rounded up to a multiple of four
+    int64_t tokens_before[PAGED_BATCH];      // of the sequences before, each rounded up to a multiple of four
 };
 // The scores of one query head: [sequence][head][positions, rounded up to a multiple of four].
 __device__ __forceinline__ float *scores_of(const AttendArgs &a, int i, int head) {
-    return a.scores + (int64_t)a.tokens_before[i] * a.q_heads + (int64_t)head * ((a.len[i] + 3) & ~3);
+    return a.scores + a.tokens_before[i] * a.q_heads + (int64_t)head * ((a.len[i] + 3) & ~3);
 }
 // The sequence that chunk `b` belongs to: how many sequences end at or before it.
 __device__ __forceinline__ int sequence_of(const AttendArgs &a, int b) {
@@ -643,10 +642,12 @@ __global__ __launch_bounds__(TPB, NE <= 8 ? 3 : 1) void paged_attend_tiles_i8_ke
     tile_finish(a, st, reinterpret_cast<float *>(shared), w.i, blockIdx.x, w.head0, w.heads, [](int j, int row) { return NE * row + j; });
 }
 
-// Joins the chunks, a workgroup per 32 values of an output row (few rows of many chunks are the case that takes long):
-// every chunk's share of the row's sum first (one thread a chunk), then W values a thread and the chunks dealt over the
-// threads that share a column, added up in a fixed order.  accumulate: the row's maximum and one over its sum are left for
-// paged_weights_kernel.
+// What follows the chunks, in one launch.  The first `joins` workgroups join them, each 32 values of an output row (few
+// rows of many chunks are the case that takes long): every chunk's share of the row's sum first (one thread a chunk), then
+// W values a thread and the chunks dealt over the threads that share a column, added up in a fixed order.  accumulate: the
+// others add the probabilities of 1024 positions of one sequence and key head, summed over its query heads, to their
+// weights, and work the row's maximum and sum out of the chunks' again (some hundred values): waiting for the joins that
+// have them would be a launch of its own, 3.5 us.
 constexpr int JOIN_CHUNKS = 1024;
 __device__ __forceinline__ float2 join_stats(const AttendArgs &a, int first, int chunks, int head, int lane) {  // by one wavefront
     float top = -INFINITY, total = 0.f;
@@ -660,14 +661,13 @@ __device__ __forceinline__ float2 join_stats(const AttendArgs &a, int first, int
     return make_float2(safe, lanes_sum<64>(total * __builtin_amdgcn_exp2f(top - safe)));
 }
 template <int W>
-__global__ __launch_bounds__(TPB) void paged_join_kernel(const AttendArgs a) {
-    __shared__ float share[JOIN_CHUNKS], sums[TPB][W];
+__device__ __forceinline__ void attend_join(const AttendArgs &a, float *share, float (*sums)[W], int row, int block) {
     const int tid = threadIdx.x, lane = tid & 63;
     constexpr int COLS = 32 / W, GROUPS = TPB / COLS;
-    const int i = blockIdx.x / a.q_heads, head = blockIdx.x - i * a.q_heads;
+    const int i = row / a.q_heads, head = row - i * a.q_heads;
     const int first = a.first[i], chunks = (a.len[i] + a.chunk[i] - 1) / a.chunk[i];
-    const float2 row = join_stats(a, first, chunks, head, lane);  // (every wavefront for itself: the same bits)
-    const int column = 32 * blockIdx.y + W * (tid % COLS), group = tid / COLS;
+    const float2 whole = join_stats(a, first, chunks, head, lane);  // (every wavefront for itself: the same bits)
+    const int column = 32 * block + W * (tid % COLS), group = tid / COLS;
     const bool live = column < a.p.d;
     float o[W];
 #pragma unroll
@@ -675,7 +675,7 @@ __global__ __launch_bounds__(TPB) void paged_join_kernel(const AttendArgs a) {
     for (int c0 = 0; c0 < chunks; c0 += JOIN_CHUNKS) {
         const int some = min(chunks - c0, JOIN_CHUNKS);
         __syncthreads();
-        for (int c = tid; c < some; c += TPB) share[c] = __builtin_amdgcn_exp2f(a.ml[(int64_t)(first + c0 + c) * a.q_heads + head].x - row.x);
+        for (int c = tid; c < some; c += TPB) share[c] = __builtin_amdgcn_exp2f(a.ml[(int64_t)(first + c0 + c) * a.q_heads + head].x - whole.x);
         __syncthreads();
         if (live) {
             const float *part = a.part + ((int64_t)(first + c0) * a.q_heads + head) * a.p.d + column;
@@ -691,31 +691,48 @@ __global__ __launch_bounds__(TPB) void paged_join_kernel(const AttendArgs a) {
 #pragma unroll
     for (int e = 0; e < W; ++e) sums[tid][e] = o[e];
     __syncthreads();
-    if (tid < 32 && 32 * (int)blockIdx.y + tid < a.p.d) {
+    if (tid < 32 && 32 * block + tid < a.p.d) {
         float sum = 0.f;
         for (int g = 0; g < GROUPS; ++g) sum += sums[g * COLS + tid / W][tid % W];
-        a.out[(int64_t)blockIdx.x * a.p.d + 32 * blockIdx.y + tid] = chunks > 0 ? sum / row.y : 0.f;
+        a.out[(int64_t)row * a.p.d + 32 * block + tid] = chunks > 0 ? sum / whole.y : 0.f;
     }
-    if (a.stats && blockIdx.y == 0 && tid == 0) a.stats[blockIdx.x] = make_float2(row.x, 1.0f / row.y);
 }
-// Adds the probabilities of 1024 positions of one sequence and key head, summed over its query heads, to their weights.
-__global__ __launch_bounds__(TPB) void paged_weights_kernel(const AttendArgs a) {
-    const int i = blockIdx.y / a.p.heads, h = blockIdx.y - i * a.p.heads, len = a.len[i];
-    const int t = 4 * (int)(blockIdx.x * TPB + threadIdx.x);
-    if (t >= len) return;
+__device__ __forceinline__ void attend_weights(const AttendArgs &a, float2 *stats, int row, int block) {
+    constexpr int WAVES = TPB / 64;
+    const int i = row / a.p.heads, h = row - i * a.p.heads, len = a.len[i], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (block * 4 * TPB >= len) return;  // (the whole workgroup)
+    const int t = 4 * (block * TPB + (int)threadIdx.x), first = a.first[i], chunks = (len + a.chunk[i] - 1) / a.chunk[i];
     f32x4 w = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int g = 0; g < a.group; ++g) {
-        const int head = h * a.group + g;
-        const float2 s = a.stats[i * a.q_heads + head];
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(scores_of(a, i, head) + t);
+    for (int g0 = 0; g0 < a.group; g0 += WAVES) {
+        const int some = min(WAVES, a.group - g0);
+        __syncthreads();
+        if (wave < some) {
+            const float2 s = join_stats(a, first, chunks, h * a.group + g0 + wave, lane);
+            if (lane == 0) stats[wave] = make_float2(s.x, 1.0f / s.y);
+        }
+        f32x4 x[WAVES];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(x[e] - s.x) * s.y;
+        for (int g = 0; g < WAVES; ++g)
+            if (t < len && g < some) x[g] = *reinterpret_cast<const f32x4 *>(scores_of(a, i, h * a.group + g0 + g) + t);
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < WAVES; ++g)
+            if (t < len && g < some) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] += __builtin_amdgcn_exp2f(x[g][e] - stats[g].x) * stats[g].y;
+            }
     }
     float *weight = a.p.weight + ((int64_t)a.slot[i] * a.p.heads + h) * a.p.max_len + t;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (t + e < len) weight[e] += w[e];
+}
+template <int W>
+__global__ __launch_bounds__(TPB) void paged_join_kernel(const AttendArgs a, int joins, int tiles) {
+    __shared__ float share[JOIN_CHUNKS], sums[TPB][W];
+    const int b = blockIdx.x, blocks = (a.p.d + 31) / 32;
+    if (b < joins) attend_join<W>(a, share, sums, b / blocks, b % blocks);
+    else attend_weights(a, reinterpret_cast<float2 *>(share), (b - joins) / tiles, (b - joins) % tiles);
 }
 
 template <bool Q8, bool VEC, int LPR, int U>
@@ -768,7 +785,6 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
     a.out = out;
     a.part = nullptr;
     a.ml = nullptr;
-    a.stats = nullptr;
     a.scores = nullptr;
     a.n = s.n;
     a.q_heads = q_heads;
@@ -796,7 +812,7 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
         a.slot[i] = i < s.n ? s.slot[i] : 0;
         a.len[i] = (int32_t)len;
         a.first[i] = i < s.n ? chunks : INT_MAX;
-        a.tokens_before[i] = (int32_t)before;
+        a.tokens_before[i] = before;
         const int64_t c = len > target ? (len + target - 1) / target : 1;  // (an empty sequence: one that writes zeros)
         int64_t chunk = (len + c - 1) / c;
         chunk = chunk > 0 ? (chunk + ATTEND_STEP - 1) / ATTEND_STEP * ATTEND_STEP : ATTEND_STEP;
@@ -807,19 +823,16 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
             chunks += (int)used;
             before += (len + 3) & ~(int64_t)3;
             if (chunk > widest) widest = chunk;
-            if (before > INT_MAX) return set_error(MNI_ERR_INVALID, "paged cache attend: more than 2^31 positions in one call");
         }
     }
     a.first[PAGED_BATCH] = INT_MAX;
-    void *part = nullptr, *ml = nullptr, *scores = nullptr, *stats = nullptr;
+    void *part = nullptr, *ml = nullptr, *scores = nullptr;
     int rc = MNI_OK;
     if (several || accumulate) {
         rc = dev_alloc(&part, (size_t)chunks * q_heads * p.d * sizeof(float));
         if (rc == MNI_OK) rc = dev_alloc(&ml, (size_t)chunks * q_heads * sizeof(float2));
         if (rc == MNI_OK && accumulate) rc = dev_alloc(&scores, (size_t)(before > 0 ? before : 1) * q_heads * sizeof(float));
-        if (rc == MNI_OK && accumulate) rc = dev_alloc(&stats, (size_t)s.n * q_heads * sizeof(float2));
         a.part = (float *)part;
-        a.stats = (float2 *)stats;
         a.ml = (float2 *)ml;
         a.scores = (float *)scores;
     }
@@ -856,19 +869,15 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
         rc = check_launch("paged_attend");
     }
     if (rc == MNI_OK && a.part) {
-        const dim3 grid((unsigned)(s.n * q_heads), (unsigned)((p.d + 31) / 32));
-        if (p.d % 4 == 0) MNI_KERNEL_LAUNCH(paged_join_kernel<4>, grid, dim3(TPB), 0, ctx().stream, a);
-        else MNI_KERNEL_LAUNCH(paged_join_kernel<1>, grid, dim3(TPB), 0, ctx().stream, a);
+        const int joins = s.n * q_heads * ((p.d + 31) / 32), tiles = (int)((longest + 4 * TPB - 1) / (4 * TPB));
+        const dim3 grid((unsigned)(joins + (accumulate ? s.n * p.heads * tiles : 0)));
+        if (p.d % 4 == 0) MNI_KERNEL_LAUNCH(paged_join_kernel<4>, grid, dim3(TPB), 0, ctx().stream, a, joins, tiles);
+        else MNI_KERNEL_LAUNCH(paged_join_kernel<1>, grid, dim3(TPB), 0, ctx().stream, a, joins, tiles);
         rc = check_launch("paged_join");
-    }
-    if (rc == MNI_OK && accumulate && longest > 0) {
-        MNI_KERNEL_LAUNCH(paged_weights_kernel, dim3((unsigned)((longest + 4 * TPB - 1) / (4 * TPB)), (unsigned)(s.n * p.heads)), dim3(TPB), 0, ctx().stream, a);
-        rc = check_launch("paged_weights");
     }
     if (part) dev_free(part);
     if (ml) dev_free(ml);
     if (scores) dev_free(scores);
-    if (stats) dev_free(stats);
     return rc;
 }
 
