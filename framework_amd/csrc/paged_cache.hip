@@ -160,7 +160,8 @@ __global__ __launch_bounds__(TPB) void paged_read_kernel(const PagedPool p, int 
 // position).  The weight becomes an ordered 32-bit key (recent rows above every key), and the last key that stays is found
 // by its digits of eight bits from the highest on, each from a histogram of the keys that share the digits before; where
 // only some of the rows with that key stay, the same search on the position tells which.  A thread holds its keys in
-// registers (up to 32768 rows; of longer sequences they are read again, from the L2), every digit has a histogram of its
+// registers (up to 16384 rows: 27 us there, 36 read again for every digit; with 32 keys a thread the registers spill, 56
+// against 52 us at 24000 rows), every digit has a histogram of its
 // own, cleared at the start, and every wavefront reads it for itself: one barrier a digit.  (Two bits a turn by ballots, with
 // nothing to collide on, took 35 us on 256 x 4608 rows.)  Then one pass in row order lists the freed places below the
 // budget and the surviving rows behind it, and paged_move_kernel moves row j of the second list to place j of the first.
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(TPB) void paged_read_kernel(const PagedPool p, int 
 constexpr int SELECT_TPB = 1024;
 struct EvictArgs {
     PagedPool p;
-    int n, budget, recent, cap;
+    int n, budget, recent, cap, lanes_log2;
     int32_t *moves;  // [n][heads][2 * cap + 1]: count, places, sources
     int32_t slot[PAGED_BATCH], len[PAGED_BATCH], seen[PAGED_BATCH];
 };
@@ -289,27 +290,28 @@ __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArg
     });
     if (tid == 0) out[0] = min(min(holes, movers), a.cap);
 }
-// A wavefront per move; blockIdx.y: (sequence, head).  Rows are stored past the caches (nontemporal): left in the last-level
-// cache they are written back under the next attention's reads (1.07 GB of rows behind 230 MB of moves and appends: 214 us
-// instead of 162; the moves themselves take 37 us either way).
+// As many lanes per move as a row has 16-byte pieces, rounded up to a power of two (other rows: 64); blockIdx.y: (sequence,
+// head).  32 x 4096 moves of 64-byte rows take 7 us so, 26 at a wavefront each; 256 x 512 of 512 bytes 32 and 37.  Rows are
+// stored past the caches (nontemporal): left in the last-level cache they are written back under the next attention's
+// reads (1.07 GB of rows behind 230 MB of moves and appends: 214 us instead of 162).
 __global__ __launch_bounds__(TPB) void paged_move_kernel(const EvictArgs a) {
     const PagedPool &p = a.p;
-    const int i = blockIdx.y / p.heads, h = blockIdx.y - i * p.heads, lane = threadIdx.x & 63;
+    const int i = blockIdx.y / p.heads, h = blockIdx.y - i * p.heads, lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
     const int32_t *moves = a.moves + (int64_t)blockIdx.y * (2 * (int64_t)a.cap + 1);
-    const int j = blockIdx.x * (TPB / 64) + (threadIdx.x >> 6);
+    const int j = blockIdx.x * (TPB >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
     if (j >= moves[0]) return;
     const int to = moves[1 + j], from = moves[1 + a.cap + j];
     const int32_t *table = p.table + a.slot[i] * p.max_pages;
     const int64_t dst = row_of(p, table[to >> p.shift], h, to & (p.page - 1)), src = row_of(p, table[from >> p.shift], h, from & (p.page - 1));
     const int bytes = p.d * (p.quantized ? 1 : 4);
     if (bytes % 16 == 0) {
-        for (int c = lane; c < bytes / 16; c += 64) {
+        for (int c = lane; c < bytes / 16; c += lanes) {
             const i32x4 k = reinterpret_cast<const i32x4 *>((const char *)p.k + src * bytes)[c], v = reinterpret_cast<const i32x4 *>((const char *)p.v + src * bytes)[c];
             __builtin_nontemporal_store(k, reinterpret_cast<i32x4 *>((char *)p.k + dst * bytes) + c);
             __builtin_nontemporal_store(v, reinterpret_cast<i32x4 *>((char *)p.v + dst * bytes) + c);
         }
     } else {
-        for (int c = lane; c < bytes; c += 64) {
+        for (int c = lane; c < bytes; c += lanes) {
             ((char *)p.k)[dst * bytes + c] = ((const char *)p.k)[src * bytes + c];
             ((char *)p.v)[dst * bytes + c] = ((const char *)p.v)[src * bytes + c];
         }
@@ -399,16 +401,20 @@ int k_paged_evict(const PagedPool &p, const PagedSeqs &s, const int32_t *seen, i
     const int64_t behind = longest - budget;
     if (s.n <= 0 || behind <= 0 || budget <= 0) return MNI_OK;
     a.cap = (int)(behind < budget ? behind : budget);  // at most so many rows change place
+    const int bytes = p.d * (p.quantized ? 1 : 4);
+    a.lanes_log2 = 0;
+    while (a.lanes_log2 < 6 && (bytes % 16 || (16 << a.lanes_log2) < bytes)) ++a.lanes_log2;
     void *moves = nullptr;
     MNI_TRY(dev_alloc(&moves, (size_t)s.n * p.heads * (2 * (size_t)a.cap + 1) * sizeof(int32_t)));
     a.moves = (int32_t *)moves;
     const dim3 grid((unsigned)(s.n * p.heads));
     if (longest <= 8 * SELECT_TPB) MNI_KERNEL_LAUNCH(paged_select_kernel<8>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
-    else if (longest <= 32 * SELECT_TPB) MNI_KERNEL_LAUNCH(paged_select_kernel<32>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
+    else if (longest <= 16 * SELECT_TPB) MNI_KERNEL_LAUNCH(paged_select_kernel<16>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
     else MNI_KERNEL_LAUNCH(paged_select_kernel<0>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
     int rc = check_launch("paged_select");
     if (rc == MNI_OK) {
-        MNI_KERNEL_LAUNCH(paged_move_kernel, dim3((unsigned)((a.cap + 3) / 4), (unsigned)(s.n * p.heads)), dim3(TPB), 0, ctx().stream, a);
+        const int per_block = TPB >> a.lanes_log2;
+        MNI_KERNEL_LAUNCH(paged_move_kernel, dim3((unsigned)((a.cap + per_block - 1) / per_block), (unsigned)(s.n * p.heads)), dim3(TPB), 0, ctx().stream, a);
         rc = check_launch("paged_move");
     }
     dev_free(moves);
