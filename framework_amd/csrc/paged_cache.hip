@@ -10,7 +10,8 @@ constexpr int TPB = 256;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // ---- page copies, forks -----------------------------------------------------------------------------
-// blockIdx.x: the copy, blockIdx.y: keys, values, key scales, value scales.  A page is one contiguous block.
+// blockIdx.x: the copy, blockIdx.y: keys, values, key scales, value scales.  A page is one contiguous block, copied in
+// pieces of 16 KB (1 MB of keys and 1 of values: 3.6 us, launch-bound).
 __global__ __launch_bounds__(TPB) void paged_copy_kernel(const PagedPool p, const PagedCopies c) {
     const int what = blockIdx.y;
     const int64_t rows = (int64_t)p.heads * p.page, unit = what >= 2 || !p.quantized ? 4 : 1;
@@ -18,12 +19,13 @@ __global__ __launch_bounds__(TPB) void paged_copy_kernel(const PagedPool p, cons
     char *base = (char *)(what == 0 ? p.k : what == 1 ? p.v : what == 2 ? (void *)p.kscale : (void *)p.vscale);
     const char *src = base + c.from[blockIdx.x] * bytes;
     char *dst = base + c.to[blockIdx.x] * bytes;
+    const int64_t first = (int64_t)blockIdx.z * TPB + threadIdx.x, step = (int64_t)gridDim.z * TPB;
     if (bytes % 16 == 0) {
-        for (int64_t i = threadIdx.x; i < bytes / 16; i += TPB) reinterpret_cast<int4 *>(dst)[i] = reinterpret_cast<const int4 *>(src)[i];
+        for (int64_t i = first; i < bytes / 16; i += step) reinterpret_cast<int4 *>(dst)[i] = reinterpret_cast<const int4 *>(src)[i];
     } else {
-        for (int64_t i = threadIdx.x; i < bytes; i += TPB) dst[i] = src[i];
+        for (int64_t i = first; i < bytes; i += step) dst[i] = src[i];
     }
-    if (what == 0 && threadIdx.x == 0) p.table[c.at[blockIdx.x]] = c.to[blockIdx.x];
+    if (what == 0 && first == 0) p.table[c.at[blockIdx.x]] = c.to[blockIdx.x];
 }
 __global__ __launch_bounds__(TPB) void paged_fork_kernel(const PagedPool p, int from, int to, int64_t len) {
     const int64_t i = (int64_t)blockIdx.x * TPB + threadIdx.x;
@@ -353,7 +355,8 @@ int paged_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
 
 int k_paged_copy(const PagedPool &p, const PagedCopies &c) {
     if (c.n <= 0) return MNI_OK;
-    MNI_KERNEL_LAUNCH(paged_copy_kernel, dim3((unsigned)c.n, p.quantized ? 4 : 2), dim3(TPB), 0, ctx().stream, p, c);
+    const int64_t bytes = (int64_t)p.heads * p.page * p.d * (p.quantized ? 1 : 4), parts = (bytes + 16383) / 16384;
+    MNI_KERNEL_LAUNCH(paged_copy_kernel, dim3((unsigned)c.n, p.quantized ? 4 : 2, (unsigned)(parts < 1024 ? parts : 1024)), dim3(TPB), 0, ctx().stream, p, c);
     return check_launch("paged_copy");
 }
 int k_paged_fork(const PagedPool &p, int32_t from, int32_t to, int64_t len) {
