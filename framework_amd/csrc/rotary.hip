@@ -1,6 +1,8 @@
 // Norm of queries and keys for each head with the rotation of their positions in the same pass, and its backward
-// (mni_rocm_qk_norm_rope).  Bandwidth-bound: 8 bytes an element forward (one read, one write), 12 backward; what the
-// chip could waste on top are the sines, so a group of lanes keeps its token's and uses them for several heads.
+// (mni_rocm_qk_norm_rope).  Bound by bandwidth where there are many rows: 8 bytes an element forward (one read, one
+// write), 12 backward, and both run at the rate of a large copy (5.6 TB/s; less than the whole traffic need reach HBM):
+// forward 5.7 TB/s on 2047 x 40 rows of 128 values (84 MB, 14.6 us), 6.2 on 8192 x 24 of 64 (101 MB, 16.2 us), backward
+// 5.8 there (151 MB, 25.8 us).  A decoding step's 8 x 24 rows are one launch, 3.7 us.  All sums are fp32, the angles 64-bit.
 #include <math.h>
 #include <string.h>
 
@@ -43,7 +45,7 @@ __device__ __forceinline__ RopePlace rope_place(const RopeArgs &a, int l) {
 }
 // cos and sin of the four pairs of a lane (pairs lo .. lo + 3; interleaved: lo / 2, lo / 2 + 1, hi / 2, hi / 2 + 1).
 // position * turns in 64 bits, less whole turns: the fraction keeps 24 good bits for any 32-bit position.
-__device__ __forceinline__ void rope_angles(const RopeArgs &a, const RopePlace &p, const double (&f)[4], uint32_t token, float (&c)[4], float (&s)[4]) {
+__device__ __forceinline__ void rope_angles(const RopeArgs &a, const double (&f)[4], uint32_t token, float (&c)[4], float (&s)[4]) {
     const uint32_t b = token / a.seq, t = token - b * a.seq;
     const double at = (double)((a.positions ? (int64_t)a.positions[b * a.position_stride + t] : (int64_t)t) + a.offset);
 #pragma unroll
@@ -93,8 +95,8 @@ __device__ __forceinline__ int64_t rope_out(const mni_rope_heads &o, const RopeA
 }
 
 // Forward.  LPR lanes hold a row; a group of LPR lanes takes the heads chunk, chunk + chunks, ... of one token (queries
-// first, then keys), HPG of them: neighbouring groups read neighbouring heads, and the HPG rows are all asked for
-// before the sines are computed.
+// first, then keys), HPG of them: neighbouring groups read neighbouring heads, the sines are computed once for the HPG
+// rows, and those are all asked for before.  (HPG is 4 from 65536 rows on, where there are groups enough for it; below, 1.)
 template <int LPR, int HPG>
 __global__ __launch_bounds__(ROPE_TPB) void rope_forward_kernel(const RopeArgs a) {
     const uint32_t item = blockIdx.x * (ROPE_TPB / LPR) + threadIdx.x / LPR;
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(ROPE_TPB) void rope_forward_kernel(const RopeArgs a
         if (h < heads) rope_load(is_q ? rope_row(a.q, a, token, h) : rope_row(a.k, a, token, h - (int)a.q.heads), p, v[j]);
     }
     float c[4], s[4];
-    rope_angles(a, p, f, token, c, s);
+    rope_angles(a, f, token, c, s);
 #pragma unroll
     for (int j = 0; j < HPG; ++j) {
         const int h = chunk + j * a.chunks;
@@ -131,9 +133,9 @@ __global__ __launch_bounds__(ROPE_TPB) void rope_forward_kernel(const RopeArgs a
     }
 }
 
-// Backward of one operand (blockIdx.y: queries, keys).  A group of lanes takes token after token and all its heads, so
-// that the sines are computed once per token and the sum for dgamma stays in registers; a workgroup leaves one partial
-// row of dgamma.
+// Backward of one operand (blockIdx.y: queries, keys).  A group of lanes takes row after row of (token, head), so that the
+// sum for dgamma stays in registers: a workgroup leaves one partial row of it, 512 at most, which one more small launch
+// adds up in order (2 us for few, 3.8 for 512; atomics would save it and make the bits a matter of chance).
 template <int LPR>
 __global__ __launch_bounds__(ROPE_TPB) void rope_backward_kernel(const RopeArgs a) {
     constexpr int GROUPS = ROPE_TPB / LPR;
@@ -148,32 +150,30 @@ __global__ __launch_bounds__(ROPE_TPB) void rope_backward_kernel(const RopeArgs 
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
     if (o.heads > 0 && o.grad) {
         rope_load(o.gamma, p, g);
-        const uint32_t items = a.tokens * a.chunks;
-        for (uint32_t item = blockIdx.x * GROUPS + group; item < items; item += gridDim.x * GROUPS) {
-            const uint32_t token = item / a.chunks;
-            float c[4], s[4];
-            rope_angles(a, p, f, token, c, s);
-            for (int h = (int)(item - token * a.chunks); h < o.heads; h += a.chunks) {
-                float x[8], dz[8];
-                rope_load(rope_row(o, a, token, h), p, x);
-                const int64_t at = rope_out(o, a, token, h);
-                rope_load(o.grad + at, p, dz);
-                float sum = 0.f, dot = 0.f;
-                if (p.turning) rope_rotate<-1>(a.interleaved, dz, c, s);
+        const uint32_t heads = (uint32_t)o.heads, rows = a.tokens * heads;
+        for (uint32_t row = blockIdx.x * GROUPS + group; row < rows; row += gridDim.x * GROUPS) {
+            const uint32_t token = row / heads;
+            const int h = (int)(row - token * heads);
+            float x[8], dz[8];
+            rope_load(rope_row(o, a, token, h), p, x);
+            const int64_t at = rope_out(o, a, token, h);
+            rope_load(o.grad + at, p, dz);
+            float c[4], s[4], sum = 0.f, dot = 0.f;
+            rope_angles(a, f, token, c, s);
+            if (p.turning) rope_rotate<-1>(a.interleaved, dz, c, s);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    sum += x[e] * x[e];
-                    dot += dz[e] * g[e] * x[e];
-                }
-                const float r = rsqrtf(lanes_sum<LPR>(sum) * a.inv_d + a.eps);
-                const float k = lanes_sum<LPR>(dot) * a.inv_d * r * r * r;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    acc[e] += dz[e] * x[e] * r;
-                    dz[e] = dz[e] * g[e] * r - x[e] * k;
-                }
-                rope_store(o.dx + at, p, dz);
+            for (int e = 0; e < 8; ++e) {
+                sum += x[e] * x[e];
+                dot += dz[e] * g[e] * x[e];
             }
+            const float r = rsqrtf(lanes_sum<LPR>(sum) * a.inv_d + a.eps);
+            const float k = lanes_sum<LPR>(dot) * a.inv_d * r * r * r;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                acc[e] += dz[e] * x[e] * r;
+                dz[e] = dz[e] * g[e] * r - x[e] * k;
+            }
+            rope_store(o.dx + at, p, dz);
         }
     }
 #pragma unroll
@@ -207,7 +207,8 @@ __global__ __launch_bounds__(1024) void rope_dgamma_kernel(const RopeArgs a, int
     }
 }
 
-// Any head_dim, rotary_dims and alignment: a wavefront per row, a lane per pair and per unrotated value.
+// Any head_dim, rotary_dims and alignment: a wavefront per row, a lane per pair and per unrotated value; 4-byte loads, and
+// rows of few values leave lanes idle.
 __device__ __forceinline__ void rope_pair(const RopeArgs &a, int i, int &lo, int &hi) {
     lo = a.interleaved ? 2 * i : i;
     hi = a.interleaved ? 2 * i + 1 : i + a.rot / 2;
@@ -384,7 +385,6 @@ int k_qk_norm_rope_backward(const mni_rope_desc &d) {
     if (empty || heads == 0 || (!d.q.grad && !d.k.grad)) return MNI_OK;
     const bool pieces = rope_in_pieces(d, true);
     const int lpr = !pieces ? 64 : a.d <= 32 ? 4 : a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32;
-    a.chunks = pieces ? (uint32_t)heads : 1;
     int64_t blocks = ((int64_t)a.tokens * heads + ROPE_TPB / lpr - 1) / (ROPE_TPB / lpr);
     if (blocks > ROPE_BWD_GROUPS) blocks = ROPE_BWD_GROUPS;
     void *part = nullptr;
