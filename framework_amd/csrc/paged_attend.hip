@@ -21,9 +21,10 @@ __device__ __forceinline__ V stream(const V *p) { return __builtin_nontemporal_l
 // (nontemporal): a decoding step comes back to a row after everything else the model holds, and 1 GB of fp32 rows is read
 // at 6.6 TB/s so, at 5.9 otherwise (79 MB that a benchmark finds in the last-level cache again: 21.5 us, 20.8 otherwise).
 //
-// paged_attend_kernel is the form for any head_dim and page: one query head, LPR lanes hold a row in 16-byte pieces (E
-// values a lane; !VEC: single values), a group of LPR lanes is a state of its own.  The keys and the values of a tile (U
-// rows each per group) are all requested before the first is used.
+// paged_attend_kernel is the vector form, for any head_dim and page: one query head, LPR lanes hold a row in 16-byte pieces
+// (E values a lane; !VEC: single values), a group of LPR lanes is a state of its own.  The keys and the values of a tile (U
+// rows each per group) are all requested before the first is used.  It reads 8 x 32 heads of 4096 fp32 rows of 96 values
+// in 119 us (6.8 TB/s) and of 256 in 321 (6.7), int8 rows of 96 in 41 (5.1); !VEC 8 x 32 x 4096 rows of 66 values in 196.
 struct AttendArgs {
     PagedPool p;
     const float *q;
@@ -370,9 +371,11 @@ __device__ __forceinline__ void tile_scores_out(const AttendArgs &a, const TileW
     }
 }
 
-// NC blocks of 64 dims (d a multiple of 4; EVEN: d = 64 NC), 16 * T positions a turn of a wavefront.  Keys of the next turn are asked for
-// when the scores are done with this turn's, values when the outputs are: every wavefront has a tile's keys or values on
-// the way at any time without a second set of registers.  The queries stay in LDS (8 reads a turn for 32 registers).
+// NC blocks of 64 dims (d a multiple of 4; EVEN: d = 64 NC), 16 * T positions a turn of a wavefront.  Keys of the next turn
+// are asked for when the scores are done with this turn's, values when the outputs are: every wavefront has a tile's keys
+// or values on the way at any time without a second set of registers.  The queries stay in LDS (8 reads a turn for 32
+// registers).  Bound by bandwidth from one query head a key head to eight: 8 x 32 heads of 4096 rows of 128 values 159 us
+// (6.75 TB/s), 192 values 242, 256 values 328 (6.5; 389 with clamped columns).
 template <int NC, int T, bool EVEN, bool WIDE>
 __global__ __launch_bounds__(TPB, NC <= 2 ? 3 : 1) void paged_attend_tiles_kernel(const AttendArgs a) {
     constexpr int WAVES = TPB / 64, TILE = 16 * T;
@@ -790,20 +793,28 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
     a.q_heads = q_heads;
     a.group = q_heads / p.heads;
     a.scale = scale * LOG2E;
-    // 16-byte pieces of a row; the matrix pipe wants them, and pages of at least four positions
-    const bool vec = p.d % (p.quantized ? 16 : 4) == 0 && ((uintptr_t)q & 15) == 0, tiles = vec && p.page >= 4;
     int64_t tokens = 0, longest = 0;
     for (int i = 0; i < s.n; ++i) {
         tokens += s.len[i];
         if (s.len[i] > longest) longest = s.len[i];
     }
+    const int64_t cus = ctx().compute_units > 0 ? ctx().compute_units : 256;
+    // 16-byte pieces of a row: both forms want them.  The matrix pipe's also wants pages of at least four positions.  Query
+    // heads that share a key head are its gain (us, 8 sequences of 4096, 32 query heads, fp32 rows of 128: 16 key heads 97,
+    // vector form 148; 8: 54 and 130).  Without them it still is as quick where its loads need no clamping and its rows no
+    // lookups (dims in 64s and pages from 16 on: fp32 159 and 161, 192 dims 242 and 238, 256 328 and 319; int8 47 and 46,
+    // 256 dims 85 and 88), else slower (96 dims 178 and 119; pages of 8, 128 dims: 198 and 164; int8, 96 dims: 45 and 41).
+    // Where the rows do not fill the chip the start and end of a workgroup count, and the vector form's are shorter for
+    // fp32 (57 rows of 12 heads: 5.4 and 4.5; 4 x 577: 6.7 and 6.1), for int8 not (4 x 2047, 12 heads: 7.2 and 8.6).
+    const bool vec = p.d % (p.quantized ? 16 : 4) == 0 && ((uintptr_t)q & 15) == 0;
+    const bool few = !p.quantized && tokens * p.heads < cus * 3 * ATTEND_LEAST;
+    const bool tiles = vec && p.page >= 4 && (a.group > 1 || (p.d % 64 == 0 && p.page >= 16 && !few));
     a.per_tile = !tiles ? 1 : p.d <= 128 ? 16 : 8;  // (the merge of 16 heads of 256 dims would not fit 64 KB of LDS)
     a.tiles_per_group = (a.group + a.per_tile - 1) / a.per_tile;
     const int64_t rows = (int64_t)p.heads * a.tiles_per_group;
-    const int64_t cus = ctx().compute_units > 0 ? ctx().compute_units : 256;
     // as many workgroups as the registers let a CU hold; scores that are kept in LDS shall take 44 KB of it at most
     const int64_t kept = 11264 / (a.group < a.per_tile ? a.group : a.per_tile) / ATTEND_STEP * ATTEND_STEP;
-    const int64_t target = attend_chunk(s, rows, tokens, cus * (p.d <= 128 ? 3 : 1), accumulate && tiles && kept < ATTEND_MOST ? kept : ATTEND_MOST);
+    const int64_t target = attend_chunk(s, rows, tokens, cus * (p.d <= 128 ? 3 : tiles ? 1 : 2), accumulate && tiles && kept < ATTEND_MOST ? kept : ATTEND_MOST);
     int chunks = 0;
     int64_t before = 0, widest = 0;
     bool several = false;
@@ -853,6 +864,9 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
             else if (p.d < 64) launch_tiles(paged_attend_tiles_kernel<1, 2, false, true>, a, chunks, w);
             else if (p.d == 128) launch_tiles(paged_attend_tiles_kernel<2, 1, true, true>, a, chunks, w);
             else if (p.d < 128) launch_tiles(paged_attend_tiles_kernel<2, 1, false, true>, a, chunks, w);
+            else if (p.d == 192) launch_tiles(paged_attend_tiles_kernel<3, 1, true, true>, a, chunks, w);
+            else if (p.d < 192) launch_tiles(paged_attend_tiles_kernel<3, 1, false, true>, a, chunks, w);
+            else if (p.d == 256) launch_tiles(paged_attend_tiles_kernel<4, 1, true, true>, a, chunks, w);
             else launch_tiles(paged_attend_tiles_kernel<4, 1, false, true>, a, chunks, w);
         } else if (tiles) {
             if (p.d <= 64) launch_tiles(paged_attend_tiles_kernel<1, 2, false, false>, a, chunks, w);
@@ -862,9 +876,14 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
             if (p.quantized) launch_attend<true, false, 64, 4>(a, chunks, w);
             else launch_attend<false, false, 64, 4>(a, chunks, w);
         } else if (p.quantized) {
-            launch_attend<true, true, 16, 4>(a, chunks, w);
+            if (p.d <= 64) launch_attend<true, true, 4, 4>(a, chunks, w);
+            else if (p.d <= 128) launch_attend<true, true, 8, 4>(a, chunks, w);
+            else launch_attend<true, true, 16, 8>(a, chunks, w);
         } else {
-            launch_attend<false, true, 64, 8>(a, chunks, w);
+            if (p.d <= 32) launch_attend<false, true, 8, 4>(a, chunks, w);
+            else if (p.d <= 64) launch_attend<false, true, 16, 4>(a, chunks, w);
+            else if (p.d <= 128) launch_attend<false, true, 32, 4>(a, chunks, w);
+            else launch_attend<false, true, 64, 8>(a, chunks, w);
         }
         rc = check_launch("paged_attend");
     }
