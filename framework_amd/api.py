@@ -337,7 +337,7 @@ def bind(native):
             native.pagedCacheTruncate(self.cacheId, seqs, lens)
 
         def attend(self, seqs, q, scale, accumulate=False):
-            return Tensor(native.pagedCacheAttend(self.cacheId, seqs, q._id, scale, accumulate))
+            return Tensor(native.pagedCacheAttend(self.cacheId, seqs, q._id, scale, accumulate), q._known_shape)
 
         def addWeights(self, seqs, w):
             native.pagedCacheAddWeights(self.cacheId, seqs, w._id)

@@ -166,20 +166,49 @@ __global__ __launch_bounds__(TPB) void paged_read_kernel(const PagedPool p, int 
 // against 52 us at 24000 rows), every digit has a histogram of its
 // own, cleared at the start, and every wavefront reads it for itself: one barrier a digit.  (Two bits a turn by ballots, with
 // nothing to collide on, took 35 us on 256 x 4608 rows.)  Then one pass in row order lists the freed places below the
-// budget and the surviving rows behind it, and paged_move_kernel moves row j of the second list to place j of the first.
+// budget and the surviving rows behind it, and row j of the second list moves to place j of the first.
 // No row is both read and written, so the move needs no order and no second buffer, and it touches only what has to
-// change place.
+// change place.  Where little moves (32 KB of keys a workgroup at most) the workgroup does it itself, with the lists in LDS;
+// more is moved by a launch of its own, with the whole chip's loads in flight (from the start of the first to the end of the
+// last, us: 48 workgroups x 77 rows of 256 bytes 10.4, in two launches 15.5; 256 x 64 of 512 bytes 16.8 and 17.2; 8 x 128 of
+// 512 16.4 and 15.8; 32 x 1024 of 64 24.1 and 21.1).
 constexpr int SELECT_TPB = 1024;
+constexpr int SELECT_LIST = 1024;  // moves whose lists take the place of the histograms
 struct EvictArgs {
     PagedPool p;
     int n, budget, recent, cap, lanes_log2;
-    int32_t *moves;  // [n][heads][2 * cap + 1]: count, places, sources
+    int32_t *moves;  // [n][heads][2 * cap + 1]: count, places, sources; null: the selection moves the rows itself
     int32_t slot[PAGED_BATCH], len[PAGED_BATCH], seen[PAGED_BATCH];
 };
 __device__ __forceinline__ uint32_t weight_key(float w, bool recent) {
     const uint32_t u = __float_as_uint(w + 0.0f);  // (-0 becomes +0)
     const uint32_t key = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
     return recent ? 0xffffffffu : w != w ? 0xfffffffeu : key;
+}
+// Row `from` of a head takes the place `to`, by `lanes` lanes.
+__device__ __forceinline__ void move_row(const EvictArgs &a, int i, int h, int to, int from, int lane, int lanes) {
+    const PagedPool &p = a.p;
+    const int32_t *table = p.table + a.slot[i] * p.max_pages;
+    const int64_t dst = row_of(p, table[to >> p.shift], h, to & (p.page - 1)), src = row_of(p, table[from >> p.shift], h, from & (p.page - 1));
+    const int bytes = p.d * (p.quantized ? 1 : 4);
+    if (bytes % 16 == 0) {
+        for (int c = lane; c < bytes / 16; c += lanes) {
+            const i32x4 k = reinterpret_cast<const i32x4 *>((const char *)p.k + src * bytes)[c], v = reinterpret_cast<const i32x4 *>((const char *)p.v + src * bytes)[c];
+            __builtin_nontemporal_store(k, reinterpret_cast<i32x4 *>((char *)p.k + dst * bytes) + c);
+            __builtin_nontemporal_store(v, reinterpret_cast<i32x4 *>((char *)p.v + dst * bytes) + c);
+        }
+    } else {
+        for (int c = lane; c < bytes; c += lanes) {
+            ((char *)p.k)[dst * bytes + c] = ((const char *)p.k)[src * bytes + c];
+            ((char *)p.v)[dst * bytes + c] = ((const char *)p.v)[src * bytes + c];
+        }
+    }
+    if (lane == 0) {
+        if (p.quantized) { p.kscale[dst] = p.kscale[src]; p.vscale[dst] = p.vscale[src]; }
+        const int64_t at = ((int64_t)a.slot[i] * p.heads + h) * p.max_len;
+        p.weight[at + to] = p.weight[at + from];
+        p.pos[at + to] = p.pos[at + from];
+    }
 }
 template <int KEYS>  // rows a thread holds: up to KEYS * SELECT_TPB in all; 0: none, they are read every time
 __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArgs a) {
@@ -188,9 +217,9 @@ __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArg
     __shared__ int waves[2][WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int i = blockIdx.x / a.p.heads, h = blockIdx.x - i * a.p.heads, len = a.len[i];
-    int32_t *out = a.moves + (int64_t)blockIdx.x * (2 * (int64_t)a.cap + 1);
+    int32_t *out = a.moves ? a.moves + (int64_t)blockIdx.x * (2 * (int64_t)a.cap + 1) : nullptr;
     if (len <= a.budget) {
-        if (tid == 0) out[0] = 0;
+        if (tid == 0 && out) out[0] = 0;
         return;
     }
     const int64_t at = ((int64_t)a.slot[i] * a.p.heads + h) * a.p.max_len;
@@ -273,6 +302,8 @@ __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArg
         late = search(digits, ties, [&](uint32_t k, int) { return k == key; }, [&](uint32_t, int t) { return (uint32_t)(top - 1 - pos[min(t, len - 1)]); }, unused,
                       unused);
     }
+    __syncthreads();  // (the histograms are read no more: they become the lists)
+    int32_t *places = out ? out + 1 : reinterpret_cast<int32_t *>(&hist[0][0]), *sources = places + a.cap;
     int holes = 0, movers = 0;
     each([&](uint32_t k, int t) {
         const bool stays = t < len && (k > key || (k == key && (late == 0 || (uint32_t)(top - 1 - pos[min(t, len - 1)]) >= late)));
@@ -286,44 +317,29 @@ __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArg
             holes += waves[0][x];
             movers += waves[1][x];
         }
-        if (hole && ho + __popcll(hb & below) < a.cap) out[1 + ho + __popcll(hb & below)] = t;
-        if (mover && mo + __popcll(mb & below) < a.cap) out[1 + a.cap + mo + __popcll(mb & below)] = t;
+        if (hole && ho + __popcll(hb & below) < a.cap) places[ho + __popcll(hb & below)] = t;
+        if (mover && mo + __popcll(mb & below) < a.cap) sources[mo + __popcll(mb & below)] = t;
         __syncthreads();
     });
-    if (tid == 0) out[0] = min(min(holes, movers), a.cap);
+    const int count = min(min(holes, movers), a.cap);
+    if (out) {
+        if (tid == 0) out[0] = count;
+        return;
+    }
+    const int lanes = 1 << a.lanes_log2;
+#pragma unroll 2
+    for (int j = tid >> a.lanes_log2; j < count; j += SELECT_TPB >> a.lanes_log2) move_row(a, i, h, places[j], sources[j], tid & (lanes - 1), lanes);
 }
 // As many lanes per move as a row has 16-byte pieces, rounded up to a power of two (other rows: 64); blockIdx.y: (sequence,
 // head).  32 x 4096 moves of 64-byte rows take 7 us so, 26 at a wavefront each; 256 x 512 of 512 bytes 32 and 37.  Rows are
 // stored past the caches (nontemporal): left in the last-level cache they are written back under the next attention's
 // reads (1.07 GB of rows behind 230 MB of moves and appends: 214 us instead of 162).
 __global__ __launch_bounds__(TPB) void paged_move_kernel(const EvictArgs a) {
-    const PagedPool &p = a.p;
-    const int i = blockIdx.y / p.heads, h = blockIdx.y - i * p.heads, lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
+    const int i = blockIdx.y / a.p.heads, h = blockIdx.y - i * a.p.heads, lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
     const int32_t *moves = a.moves + (int64_t)blockIdx.y * (2 * (int64_t)a.cap + 1);
     const int j = blockIdx.x * (TPB >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
     if (j >= moves[0]) return;
-    const int to = moves[1 + j], from = moves[1 + a.cap + j];
-    const int32_t *table = p.table + a.slot[i] * p.max_pages;
-    const int64_t dst = row_of(p, table[to >> p.shift], h, to & (p.page - 1)), src = row_of(p, table[from >> p.shift], h, from & (p.page - 1));
-    const int bytes = p.d * (p.quantized ? 1 : 4);
-    if (bytes % 16 == 0) {
-        for (int c = lane; c < bytes / 16; c += lanes) {
-            const i32x4 k = reinterpret_cast<const i32x4 *>((const char *)p.k + src * bytes)[c], v = reinterpret_cast<const i32x4 *>((const char *)p.v + src * bytes)[c];
-            __builtin_nontemporal_store(k, reinterpret_cast<i32x4 *>((char *)p.k + dst * bytes) + c);
-            __builtin_nontemporal_store(v, reinterpret_cast<i32x4 *>((char *)p.v + dst * bytes) + c);
-        }
-    } else {
-        for (int c = lane; c < bytes; c += lanes) {
-            ((char *)p.k)[dst * bytes + c] = ((const char *)p.k)[src * bytes + c];
-            ((char *)p.v)[dst * bytes + c] = ((const char *)p.v)[src * bytes + c];
-        }
-    }
-    if (lane == 0) {
-        if (p.quantized) { p.kscale[dst] = p.kscale[src]; p.vscale[dst] = p.vscale[src]; }
-        const int64_t at = ((int64_t)a.slot[i] * p.heads + h) * p.max_len;
-        p.weight[at + to] = p.weight[at + from];
-        p.pos[at + to] = p.pos[at + from];
-    }
+    move_row(a, i, h, moves[1 + j], moves[1 + a.cap + j], lane, lanes);
 }
 
 template <bool Q8, bool VEC, int LPR, class Batch>
@@ -407,20 +423,21 @@ int k_paged_evict(const PagedPool &p, const PagedSeqs &s, const int32_t *seen, i
     const int bytes = p.d * (p.quantized ? 1 : 4);
     a.lanes_log2 = 0;
     while (a.lanes_log2 < 6 && (bytes % 16 || (16 << a.lanes_log2) < bytes)) ++a.lanes_log2;
+    const bool fused = a.cap <= SELECT_LIST && (int64_t)a.cap * bytes <= 32768;
     void *moves = nullptr;
-    MNI_TRY(dev_alloc(&moves, (size_t)s.n * p.heads * (2 * (size_t)a.cap + 1) * sizeof(int32_t)));
+    if (!fused) MNI_TRY(dev_alloc(&moves, (size_t)s.n * p.heads * (2 * (size_t)a.cap + 1) * sizeof(int32_t)));
     a.moves = (int32_t *)moves;
     const dim3 grid((unsigned)(s.n * p.heads));
     if (longest <= 8 * SELECT_TPB) MNI_KERNEL_LAUNCH(paged_select_kernel<8>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
     else if (longest <= 16 * SELECT_TPB) MNI_KERNEL_LAUNCH(paged_select_kernel<16>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
     else MNI_KERNEL_LAUNCH(paged_select_kernel<0>, grid, dim3(SELECT_TPB), 0, ctx().stream, a);
     int rc = check_launch("paged_select");
-    if (rc == MNI_OK) {
+    if (rc == MNI_OK && !fused) {
         const int per_block = TPB >> a.lanes_log2;
         MNI_KERNEL_LAUNCH(paged_move_kernel, dim3((unsigned)((a.cap + per_block - 1) / per_block), (unsigned)(s.n * p.heads)), dim3(TPB), 0, ctx().stream, a);
         rc = check_launch("paged_move");
     }
-    dev_free(moves);
+    if (moves) dev_free(moves);
     return rc;
 }
 
