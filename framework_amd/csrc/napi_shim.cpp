@@ -355,45 +355,81 @@ napi_value PagedCacheSeen(napi_env env, napi_callback_info info) {
     Args a(env, info);
     return ret_count(env, mni_paged_cache_seen(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
 }
+// A list of ids or lengths: an array, or a typed array of 32-bit integers or doubles.  Anything else throws (false).
+template <class V>
+bool get_list(napi_env env, napi_value v, std::vector<V> *out, const char *what) {
+    bool is = false;
+    if (napi_is_array(env, v, &is) == napi_ok && is) {
+        uint32_t n = 0;
+        napi_get_array_length(env, v, &n);
+        out->resize(n);
+        for (uint32_t i = 0; i < n; ++i) {
+            napi_value e;
+            napi_get_element(env, v, i, &e);
+            (*out)[i] = (V)get_i64(env, e);
+        }
+        return true;
+    }
+    napi_typedarray_type type;
+    size_t n = 0;
+    void *data = nullptr;
+    if (napi_is_typedarray(env, v, &is) == napi_ok && is && napi_get_typedarray_info(env, v, &type, &n, &data, nullptr, nullptr) == napi_ok) {
+        auto copy = [&](auto *from) { out->resize(n); for (size_t i = 0; i < n; ++i) (*out)[i] = (V)from[i]; return true; };
+        if (type == napi_uint32_array) return copy((const uint32_t *)data);
+        if (type == napi_int32_array) return copy((const int32_t *)data);
+        if (type == napi_float64_array) return copy((const double *)data);
+    }
+    napi_throw_error(env, nullptr, what);
+    return false;
+}
 napi_value throw_lengths(napi_env env, const char *what) {
     napi_throw_error(env, nullptr, what);
     return nullptr;
 }
+constexpr const char *WANT_SEQS = "paged cache: an array of sequence ids is wanted";
 napi_value PagedCacheAppend(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    std::vector<uint32_t> seqs;
+    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
     const bool some = is_given(env, a.v[4]);
-    const std::vector<int64_t> counts = some ? get_i64_array(env, a.v[4]) : std::vector<int64_t>();
+    std::vector<int64_t> counts;
+    if (some && !get_list(env, a.v[4], &counts, "paged cache append: an array of counts is wanted")) return nullptr;
     if (some && counts.size() != seqs.size()) return throw_lengths(env, "paged cache append: as many counts as sequences are wanted");
     return ret_rc(env, mni_paged_cache_append(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2]), get_u32(env, a.v[3]),
                                               some ? counts.data() : nullptr));
 }
 napi_value PagedCacheTruncate(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
-    const std::vector<int64_t> lens = get_i64_array(env, a.v[2]);
+    std::vector<uint32_t> seqs;
+    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
+    std::vector<int64_t> lens;
+    if (!get_list(env, a.v[2], &lens, "paged cache truncate: an array of lengths is wanted")) return nullptr;
     if (lens.size() != seqs.size()) return throw_lengths(env, "paged cache truncate: as many lengths as sequences are wanted");
     return ret_rc(env, mni_paged_cache_truncate(get_u32(env, a.v[0]), seqs.data(), seqs.size(), lens.data()));
 }
 napi_value PagedCacheAttend(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    std::vector<uint32_t> seqs;
+    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
     return ret_id(env, mni_paged_cache_attend(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2]), get_f64(env, a.v[3]),
                                               get_bool(env, a.v[4]) ? 1 : 0));
 }
 napi_value PagedCacheAddWeights(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    std::vector<uint32_t> seqs;
+    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
     return ret_rc(env, mni_paged_cache_add_weights(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2])));
 }
 napi_value PagedCacheEvict(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    std::vector<uint32_t> seqs;
+    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
     return ret_rc(env, mni_paged_cache_evict(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_i64(env, a.v[2]), get_i64(env, a.v[3])));
 }
 napi_value PagedCacheTrack(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    const std::vector<uint32_t> seqs = get_u32_array(env, a.v[1]);
+    std::vector<uint32_t> seqs;
+    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
     uint32_t w = 0, p = 0;
     const int rc = mni_paged_cache_track(get_u32(env, a.v[0]), seqs.data(), seqs.size(), &w, &p);
     return ret_ids(env, rc, w, p);

@@ -1,0 +1,19 @@
+"""qkNormRope and the paged cache called from JavaScript through the Node-API shim."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.gpu
+def test_paged_decoding_through_the_addon():
+    node = shutil.which("node")
+    if node is None:
+        pytest.skip("no node binary on this machine")
+    if not os.path.exists(os.path.join(ROOT, "framework_amd", "lib", "mni_rocm.node")):
+        pytest.skip("Node addon not built (node_api.h missing at build time)")
+    p = subprocess.run([node, os.path.join(ROOT, "tests", "js", "paged_decode.js")], capture_output=True, text=True, timeout=100)
+    assert p.returncode == 0 and "0 failed" in p.stdout, p.stdout + p.stderr
