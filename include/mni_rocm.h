@@ -462,11 +462,12 @@ int mni_qk_norm_rope(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k,
  * len: tokens held; seen: tokens appended less those truncated (the rotation position of the next one; eviction does
  *   not change it); free_pages: pages that no sequence holds.  < 0 for an unknown id.
  * append: k, v [n, kv_heads, T, head_dim] (views welcome): sequence seqs[i] takes its first counts[i] <= T tokens, or
- *   all T where counts is NULL.  A sequence may not occur twice.
+ *   all T where counts is NULL.  A sequence may not occur twice, kv_heads * T may not pass 2^24.  Only rows behind a
+ *   sequence's end are written; a call that is refused has changed nothing.
  * truncate: back to lens[i] rows, the tokens appended last leave first (rejected drafts).  Of a sequence that has
  *   been evicted only tokens appended since then can leave this way.
  * attend: q [n, heads, 1, head_dim] (or [n * heads, 1, head_dim]) attends over everything seqs[i] holds: softmax(scale
- *   q k^T) v, in q's shape; zeros where a sequence holds nothing.  `accumulate` (tracked caches): every position's
+ *   q k^T) v, in q's shape; zeros where a sequence holds nothing; at most 4096 heads.  `accumulate` (tracked caches): every position's
  *   probability, summed over the query heads of its key head, is added to its weight; a sequence may then not occur
  *   twice.
  * add_weights: w [n, kv_heads, L], L at least the longest of them: w[i, h, j] is added to the weight of row j.
@@ -478,7 +479,9 @@ int mni_qk_norm_rope(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k,
  * track: the weights, as a tensor [n, kv_heads, longest], and the positions, as an int buffer of as many values, of
  *   every row in the order held; 0 and -1 behind a sequence's end.
  * read: keys and values of one sequence in the order held, [kv_heads, len, head_dim] (int8 rows as the values they
- *   stand for). */
+ *   stand for).
+ * Like mni_kv_cache_*, these are for answering: nothing is recorded on the tape.  Scores, maxima, sums and outputs are
+ * fp32; an int8 row is stored as round(x (1 / s)) with s = max |x| (1 / 127), at least 1e-8, each step in fp32. */
 uint32_t mni_paged_cache_create(int64_t max_sequences, int64_t max_seq_len, int64_t num_pages, int64_t page_size, int64_t kv_heads,
                                 int64_t head_dim, int quantized, int tracked);
 void mni_paged_cache_free(uint32_t cache_id);
