@@ -800,15 +800,16 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
     }
     const int64_t cus = ctx().compute_units > 0 ? ctx().compute_units : 256;
     // 16-byte pieces of a row: both forms want them.  The matrix pipe's also wants pages of at least four positions.  Query
-    // heads that share a key head are its gain (us, 8 sequences of 4096, 32 query heads, fp32 rows of 128: 16 key heads 97,
-    // vector form 148; 8: 54 and 130).  Without them it still is as quick where its loads need no clamping and its rows no
+    // heads that share a key head are its gain (us, 8 sequences of 4096, 32 query heads, fp32 rows of 128: 16 key heads 83,
+    // vector form 110; 8: 45 and 90; int8 18 and 41).  Without them it still is as quick where its loads need no clamping and its rows no
     // lookups (dims in 64s and pages from 16 on: fp32 159 and 161, 192 dims 242 and 238, 256 328 and 319; int8 47 and 46,
-    // 256 dims 85 and 88), else slower (96 dims 178 and 119; pages of 8, 128 dims: 198 and 164; int8, 96 dims: 45 and 41).
+    // 256 dims 85 and 88), else slower (96 dims 178 and 119; pages of 8, 128 dims: 198 and 164; int8, 96 dims: 45 and 41);
+    // fp32 rows of other dims than 64s even for two heads (96: 87 and 81, 32: 40 and 29; three heads of 96: 50 and 57).
     // Where the rows do not fill the chip the start and end of a workgroup count, and the vector form's are shorter for
     // fp32 (57 rows of 12 heads: 5.4 and 4.5; 4 x 577: 6.7 and 6.1), for int8 not (4 x 2047, 12 heads: 7.2 and 8.6).
     const bool vec = p.d % (p.quantized ? 16 : 4) == 0 && ((uintptr_t)q & 15) == 0;
     const bool few = !p.quantized && tokens * p.heads < cus * 3 * ATTEND_LEAST;
-    const bool tiles = vec && p.page >= 4 && (a.group > 1 || (p.d % 64 == 0 && p.page >= 16 && !few));
+    const bool tiles = vec && p.page >= 4 && (a.group > (p.quantized || p.d % 64 == 0 ? 1 : 2) || (p.d % 64 == 0 && p.page >= 16 && !few));
     a.per_tile = !tiles ? 1 : p.d <= 128 ? 16 : 8;  // (the merge of 16 heads of 256 dims would not fit 64 KB of LDS)
     a.tiles_per_group = (a.group + a.per_tile - 1) / a.per_tile;
     const int64_t rows = (int64_t)p.heads * a.tiles_per_group;
