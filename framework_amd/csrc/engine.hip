@@ -2010,6 +2010,7 @@ static uint32_t paged_create(int64_t max_sequences, int64_t max_seq_len, int64_t
     if (quantized && (!(p.kscale = (float *)block(rows * 4)) || !(p.vscale = (float *)block(rows * 4)))) return MNI_BAD_ID;
     if (!(p.table = (int32_t *)block((size_t)(max_sequences * p.max_pages) * 4))) return MNI_BAD_ID;
     if (tracked && (!(p.weight = (float *)block(track * 4)) || !(p.pos = (int32_t *)block(track * 4)))) return MNI_BAD_ID;
+    if (!(p.tickets = (int32_t *)block(PAGED_TICKETS * 4)) || k_fill((float *)p.tickets, 0.0f, PAGED_TICKETS) != MNI_OK) return MNI_BAD_ID;
     c.holders.assign((size_t)num_pages, 0);
     c.free_pages.reserve((size_t)num_pages);
     for (int64_t i = num_pages; i-- > 0;) c.free_pages.push_back((int32_t)i);

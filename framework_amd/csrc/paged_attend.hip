@@ -32,6 +32,7 @@ struct AttendArgs {
     float *part;    // [chunk of the launch][q_heads][d]: sums not yet divided (null: every sequence is one chunk)
     float2 *ml;     // [chunk of the launch][q_heads]: maximum and sum
     float *scores;  // accumulate: see scores_of
+    int32_t *tickets;  // the last workgroup of a row joins its chunks (null: paged_join_kernel does)
     int n, q_heads, group, tiles_per_group, per_tile;
     int staged;  // words of LDS that page ids take before the scores that are kept there
     float scale;  // times log2 e
@@ -85,6 +86,9 @@ struct AttendRow {  // what a lane holds of a row, as it was loaded
         }
     }
 };
+// Stores and loads that other dies see, past this one's L2.
+__device__ __forceinline__ void put_through(float *p, float x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float get_through(const float *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 // The states that the wavefronts of a workgroup left in LDS ([head][wave][d] sums, [head][wave] maxima and sums) become the
 // output, or the chunk's part of it.
 template <int WAVES>
@@ -103,12 +107,69 @@ __device__ __forceinline__ void attend_merge(const AttendArgs &a, const float *s
             o += so[(g * WAVES + w) * d + c] * f;
             total += ss[g * WAVES + w] * f;
         }
-        if (!a.part) {
+        if (!a.part || (a.tickets && a.len[i] <= a.chunk[i])) {
             a.out[((int64_t)i * a.q_heads + head0 + g) * d + c] = a.len[i] > 0 ? o / total : 0.f;
+        } else if (a.tickets) {
+            put_through(&a.part[((int64_t)b * a.q_heads + head0 + g) * d + c], o);
+            if (c == 0) {
+                float *ml = reinterpret_cast<float *>(&a.ml[(int64_t)b * a.q_heads + head0 + g]);
+                put_through(ml, top);
+                put_through(ml + 1, total);
+            }
         } else {
             a.part[((int64_t)b * a.q_heads + head0 + g) * d + c] = o;
             if (c == 0) a.ml[(int64_t)b * a.q_heads + head0 + g] = make_float2(top, total);
         }
+    }
+}
+// Few rows of few chunks are joined by the workgroup that ends last.  Chunks of a row end on different dies, whose L2s do
+// not see each other's lines: parts are stored past them (put_through), a workgroup takes its ticket when all its stores
+// have arrived, and the one with the last ticket reads past its L2.  The chunks are added in order, whoever comes last.
+// The ticket goes back to zero for the next launch.  The device takes as long as with the join's launch (48 rows of 577: 9.2
+// us, 6.1 + 3.8 apart; 256 rows of 4096 int8 50.4, 46.6 + 4.6; of fp32 168, 162 + 5), but the host starts one less: where
+// the rows do not fill the chip it is the host that a step waits for (a step with eviction over those 48 rows: 36.5 -> 31.8).
+constexpr int LAST_CHUNKS = 8;
+__device__ __forceinline__ void attend_last(const AttendArgs &a, int i, int head0, int heads) {
+    __shared__ float share[16][LAST_CHUNKS], sums[16];
+    __shared__ int taken;
+    const int chunks = (a.len[i] + a.chunk[i] - 1) / a.chunk[i], d = a.p.d, tid = threadIdx.x;
+    if (!a.tickets || chunks <= 1) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wavefront's stores have arrived
+    __syncthreads();
+    int32_t *ticket = a.tickets + i * (int)gridDim.y + (int)blockIdx.y;
+    if (tid == 0) taken = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (taken != chunks - 1) return;
+    if (tid == 0) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int64_t first = a.first[i];
+    if (tid < heads) {
+        const float *ml = reinterpret_cast<const float *>(a.ml + first * a.q_heads + head0 + tid);
+        float m[LAST_CHUNKS], s[LAST_CHUNKS], top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int c = 0; c < LAST_CHUNKS; ++c) {
+            const int64_t at = 2 * (int64_t)min(c, chunks - 1) * a.q_heads;
+            m[c] = get_through(ml + at);
+            s[c] = get_through(ml + at + 1);
+        }
+#pragma unroll
+        for (int c = 0; c < LAST_CHUNKS; ++c) top = fmaxf(top, m[c]);
+        const float safe = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int c = 0; c < LAST_CHUNKS; ++c) {
+            const float f = c < chunks ? __builtin_amdgcn_exp2f(m[c] - safe) : 0.f;
+            share[tid][c] = f;
+            if (c < chunks) total += s[c] * f;
+        }
+        sums[tid] = total;
+    }
+    __syncthreads();
+    for (int j = tid; j < heads * d; j += TPB) {
+        const int g = j / d;
+        const float *part = a.part + (first * a.q_heads + head0) * d + j;
+        float o = 0.f;
+#pragma unroll 8
+        for (int c = 0; c < chunks; ++c) o += get_through(part + (int64_t)c * a.q_heads * d) * share[g][c];
+        a.out[((int64_t)i * a.q_heads + head0) * d + j] = o / sums[g];
     }
 }
 template <bool VEC, int E>
@@ -199,6 +260,7 @@ __global__ __launch_bounds__(TPB) void paged_attend_kernel(const AttendArgs a) {
     }
     __syncthreads();
     attend_merge<WAVES>(a, so, sm, ss, i, b, head, 1);
+    attend_last(a, i, head, 1);
 }
 
 // ---- the same on the matrix pipe -----------------------------------------------------------------------------------
@@ -322,6 +384,7 @@ __device__ __forceinline__ void tile_finish(const AttendArgs &a, TileState<N> &s
     }
     __syncthreads();
     attend_merge<WAVES>(a, so, sm, ss, i, b, head0, heads);
+    attend_last(a, i, head0, heads);
 }
 // What both kernels begin with.
 struct TileWork {
@@ -789,6 +852,7 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
     a.part = nullptr;
     a.ml = nullptr;
     a.scores = nullptr;
+    a.tickets = nullptr;
     a.n = s.n;
     a.q_heads = q_heads;
     a.group = q_heads / p.heads;
@@ -808,8 +872,8 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
     // Where the rows do not fill the chip the start and end of a workgroup count, and the vector form's are shorter for
     // fp32 (57 rows of 12 heads: 5.4 and 4.5; 4 x 577: 6.7 and 6.1), for int8 not (4 x 2047, 12 heads: 7.2 and 8.6).
     const bool vec = p.d % (p.quantized ? 16 : 4) == 0 && ((uintptr_t)q & 15) == 0;
-    const bool few = !p.quantized && tokens * p.heads < cus * 3 * ATTEND_LEAST;
-    const bool tiles = vec && p.page >= 4 && (a.group > (p.quantized || p.d % 64 == 0 ? 1 : 2) || (p.d % 64 == 0 && p.page >= 16 && !few));
+    const bool few = tokens * p.heads < cus * 3 * ATTEND_LEAST;
+    const bool tiles = vec && p.page >= 4 && (a.group > (p.quantized || p.d % 64 == 0 ? 1 : 2) || (p.d % 64 == 0 && p.page >= 16 && (p.quantized || !few)));
     a.per_tile = !tiles ? 1 : p.d <= 128 ? 16 : 8;  // (the merge of 16 heads of 256 dims would not fit 64 KB of LDS)
     a.tiles_per_group = (a.group + a.per_tile - 1) / a.per_tile;
     const int64_t rows = (int64_t)p.heads * a.tiles_per_group;
@@ -818,7 +882,7 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
     const int64_t target = attend_chunk(s, rows, tokens, cus * (p.d <= 128 ? 3 : tiles ? 1 : 2), accumulate && tiles && kept < ATTEND_MOST ? kept : ATTEND_MOST);
     int chunks = 0;
     int64_t before = 0, widest = 0;
-    bool several = false;
+    int64_t most = 0;  // chunks of a row
     for (int i = 0; i < PAGED_BATCH; ++i) {
         const int64_t len = i < s.n ? s.len[i] : 0;
         a.slot[i] = i < s.n ? s.slot[i] : 0;
@@ -831,7 +895,7 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
         a.chunk[i] = (int32_t)chunk;
         if (i < s.n) {
             const int64_t used = len > 0 ? (len + chunk - 1) / chunk : 1;
-            several = several || used > 1;
+            if (used > most) most = used;
             chunks += (int)used;
             before += (len + 3) & ~(int64_t)3;
             if (chunk > widest) widest = chunk;
@@ -840,7 +904,9 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
     a.first[PAGED_BATCH] = INT_MAX;
     void *part = nullptr, *ml = nullptr, *scores = nullptr;
     int rc = MNI_OK;
-    if (several || accumulate) {
+    const bool last = few && !accumulate && most <= LAST_CHUNKS && s.n * rows <= PAGED_TICKETS;
+    if (most > 1 || accumulate) {
+        if (last) a.tickets = p.tickets;
         rc = dev_alloc(&part, (size_t)chunks * q_heads * p.d * sizeof(float));
         if (rc == MNI_OK) rc = dev_alloc(&ml, (size_t)chunks * q_heads * sizeof(float2));
         if (rc == MNI_OK && accumulate) rc = dev_alloc(&scores, (size_t)(before > 0 ? before : 1) * q_heads * sizeof(float));
@@ -888,7 +954,7 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
         }
         rc = check_launch("paged_attend");
     }
-    if (rc == MNI_OK && a.part) {
+    if (rc == MNI_OK && a.part && !last) {
         const int joins = s.n * q_heads * ((p.d + 31) / 32), tiles = (int)((longest + 4 * TPB - 1) / (4 * TPB));
         const dim3 grid((unsigned)(joins + (accumulate ? s.n * p.heads * tiles : 0)));
         if (p.d % 4 == 0) MNI_KERNEL_LAUNCH(paged_join_kernel<4>, grid, dim3(TPB), 0, ctx().stream, a, joins, tiles);

@@ -7,12 +7,14 @@ namespace mni {
 // Device side.  Row (page, head, slot) of the pool holds head_dim values of one position, fp32 or int8 with a scale;
 // table[sequence][i] is the page of positions i * page .. (i + 1) * page - 1; weight / pos (tracked caches) are kept
 // per sequence, [sequence][head][row], because a page may be shared by sequences that weigh it differently.
+constexpr int PAGED_TICKETS = 16384;
 struct PagedPool {
     void *k, *v;
     float *kscale, *vscale;  // quantized only
     int32_t *table;
     float *weight;           // tracked only
     int32_t *pos;
+    int32_t *tickets;        // [PAGED_TICKETS], zeros between launches: see attend_last
     int64_t max_pages, max_len;
     int heads, d, page, shift, quantized;
 };

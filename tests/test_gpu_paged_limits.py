@@ -168,3 +168,29 @@ def test_two_threads(gpu):
                 m.append(rows[t][1][j][i], rows[t][2][j][i], False)
                 want, tol, _ = m.attend(rows[t][0][j][i, :, 0], 0.125, False)
                 assert (np.abs(out[t][j][i, :, 0] - want) <= tol[:, None]).all()
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("heads,group,d,page", [(12, 1, 64, 16), (2, 4, 128, 16), (3, 2, 7, 8)])
+def test_the_same_bits_whichever_workgroup_ends_last(gpu, heads, group, d, page, quantized):
+    """Rows of one to nine chunks: every call gives the first one's bits, and the first one's are right."""
+    lens = [1, 64, 128, 129, 300, 577, 1024, 1100]
+    n = len(lens)
+    cache = gpu.PagedKvCache(n, 1152, sum(-(-x // page) for x in lens), page, heads, d, quantized=quantized)
+    seqs, models = [cache.add() for _ in lens], [Model(heads, d) for _ in lens]
+    k, v = (synth.normal(1 + i, (n, heads, max(lens), d), stream=i) for i in range(2))
+    cache.append(seqs, _t(gpu, k), _t(gpu, v), lens)
+    q = synth.normal(3, (n, heads * group, 1, d))
+    q_t = _t(gpu, q)
+    first = cache.attend(seqs, q_t, 0.2).numpy()
+    for i, m in enumerate(models):
+        m.append(k[i, :, :lens[i]], v[i, :, :lens[i]], quantized)
+        want, tol, _ = m.attend(q[i, :, 0], 0.2, False)
+        assert (np.abs(first[i, :, 0] - want) <= tol[:, None]).all(), lens[i]
+    outs = [cache.attend(seqs, q_t, 0.2) for _ in range(150)]  # queued one behind the other
+    assert all(np.array_equal(o.numpy(), first) for o in outs)
+    # one sequence alone is cut into other chunks: as right, not the same bits
+    for i, m in enumerate(models):
+        got = cache.attend([seqs[i]], _t(gpu, q[i:i + 1]), 0.2).numpy()
+        want, tol, _ = m.attend(q[i, :, 0], 0.2, False)
+        assert (np.abs(got[0, :, 0] - want) <= tol[:, None]).all(), lens[i]
