@@ -194,3 +194,45 @@ def test_the_same_bits_whichever_workgroup_ends_last(gpu, heads, group, d, page,
         got = cache.attend([seqs[i]], _t(gpu, q[i:i + 1]), 0.2).numpy()
         want, tol, _ = m.attend(q[i, :, 0], 0.2, False)
         assert (np.abs(got[0, :, 0] - want) <= tol[:, None]).all(), lens[i]
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("heads,group,d,page", [(1, 40, 64, 16), (2, 17, 128, 64), (1, 33, 256, 16), (2, 19, 80, 4), (1, 20, 20, 1)])
+def test_more_query_heads_than_a_tile_holds(gpu, heads, group, d, page, quantized):
+    lens = [3, 700, 0, 131]
+    cache = gpu.PagedKvCache(4, 704, sum(-(-x // page) for x in lens), page, heads, d, quantized=quantized, tracked=True)
+    seqs, models = [cache.add() for _ in lens], [Model(heads, d) for _ in lens]
+    k, v = (synth.normal(1 + i, (4, heads, 700, d), stream=i) for i in range(2))
+    cache.append(seqs, _t(gpu, k), _t(gpu, v), lens)
+    q = synth.normal(3, (4, heads * group, 1, d))
+    plain = cache.attend(seqs, _t(gpu, q), 0.1).numpy()
+    got = cache.attend(seqs, _t(gpu, q), 0.1, accumulate=True).numpy()
+    weights = cache.track(seqs)[0].numpy()
+    for i, m in enumerate(models):
+        m.append(k[i, :, :lens[i]], v[i, :, :lens[i]], quantized)
+        want, tol, wtol = m.attend(q[i, :, 0], 0.1, True)
+        for out in (plain, got):
+            assert (np.abs(out[i, :, 0] - want) <= tol[:, None]).all(), i
+        assert (np.abs(weights[i, :, :lens[i]] - np.stack(m.w)) <= wtol + 4 * U).all() and (weights[i, :, lens[i]:] == 0).all()
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("heads,group,d,page,lens", [  # rows that fill the chip, and every width of a tile
+    (16, 1, 64, 16, [7000]), (16, 1, 128, 64, [3500, 2701]), (16, 1, 192, 32, [6200]), (32, 1, 256, 16, [3111]),
+    (4, 3, 192, 16, [900, 33]), (2, 3, 160, 32, [701]), (2, 2, 224, 16, [500, 1]), (3, 2, 192, 8, [300]), (2, 2, 36, 16, [200, 17])])
+def test_every_form_of_attention(gpu, heads, group, d, page, lens, quantized):
+    n, longest = len(lens), max(lens)
+    cache = gpu.PagedKvCache(n, longest, sum(-(-x // page) for x in lens), page, heads, d, quantized=quantized, tracked=True)
+    seqs, models = [cache.add() for _ in lens], [Model(heads, d) for _ in lens]
+    k, v = (synth.normal(1 + i, (n, heads, longest, d), stream=i) for i in range(2))
+    cache.append(seqs, _t(gpu, k), _t(gpu, v), lens)
+    q = synth.normal(3, (n, heads * group, 1, d))
+    plain = cache.attend(seqs, _t(gpu, q), 0.08).numpy()
+    got = cache.attend(seqs, _t(gpu, q), 0.08, accumulate=True).numpy()
+    weights = cache.track(seqs)[0].numpy()
+    for i, m in enumerate(models):
+        m.append(k[i, :, :lens[i]], v[i, :, :lens[i]], quantized)
+        want, tol, wtol = m.attend(q[i, :, 0], 0.08, True)
+        for out in (plain, got):
+            assert (np.abs(out[i, :, 0] - want) <= tol[:, None]).all(), i
+        assert (np.abs(weights[i, :, :lens[i]] - np.stack(m.w)) <= wtol + 4 * U).all()
