@@ -43,7 +43,7 @@ __global__ __launch_bounds__(TPB) void paged_fork_kernel(const PagedPool p, int 
 // round(x * (1 / scale)), halves away from zero: a stored value is at most half a scale off, and no code leaves -127 .. 127
 // (the largest is 127 to three roundings).  (The contiguous cache divides by 127; the two scales differ by one rounding.)
 // VEC: 4 values per lane, else one value per lane and turn.  Bound by bandwidth: 134 MB of fp32 rows read and written in 46
-// us (5.8 TB/s, the rate of a large copy), 31 MB stored as 8 MB of int8 rows in 10.2.
+// us (5.8 TB/s, the rate of a large copy), 31 MB stored as 8 MB of int8 rows in 9.5.
 template <bool VEC>
 struct AppendRow {
     static constexpr int N = VEC ? 1 : 4;  // pieces per lane (d <= 256)
@@ -79,12 +79,19 @@ struct AppendRow {
         float scale = mx * (1.0f / 127.0f);
         if (!(scale > 1e-8f)) scale = 1e-8f;
         const float inv = 1.0f / scale;
-        auto code = [&](float v) { return (int)roundf(v * inv); };
+        // halves away from zero: the whole part of y and, towards its sign, the largest value below a half (what round() gives
+        // for every |y| up to 128; the product is rounded before the sum, which a fused multiply-add would not do)
+        auto code = [&](float v) {
+#pragma clang fp contract(off)
+            const float y = v * inv;
+            return (int)(y + copysignf(0.49999997f, y));
+        };
         signed char *dst = (signed char *)cache + row * d;
         if (VEC) {
             if (4 * l < d)
-                *reinterpret_cast<uint32_t *>(dst + 4 * l) = (uint32_t)(code(x[0].x) & 255) | (uint32_t)(code(x[0].y) & 255) << 8 |
-                                                             (uint32_t)(code(x[0].z) & 255) << 16 | (uint32_t)(code(x[0].w) & 255) << 24;
+                *reinterpret_cast<uint32_t *>(dst + 4 * l) =
+                    __builtin_amdgcn_perm((uint32_t)code(x[0].w), (uint32_t)code(x[0].z), 0x04000c0c) |
+                    __builtin_amdgcn_perm((uint32_t)code(x[0].y), (uint32_t)code(x[0].x), 0x0c0c0400);
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
