@@ -236,3 +236,24 @@ def test_every_form_of_attention(gpu, heads, group, d, page, lens, quantized):
         for out in (plain, got):
             assert (np.abs(out[i, :, 0] - want) <= tol[:, None]).all(), i
         assert (np.abs(weights[i, :, :lens[i]] - np.stack(m.w)) <= wtol + 4 * U).all()
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("lens,budget,recent,d", [([20000], 19800, 90, 16), ([16384, 9000], 8999, 8, 7), ([16385], 16384, 0, 4), ([700, 20, 650], 600, 40, 128),
+                                                  ([700, 20, 650], 300, 40, 100)])
+def test_eviction_by_the_selection_itself_and_by_moves(gpu, lens, budget, recent, d, quantized):
+    """Few and many bytes to move, rows of every kind of width, sequences that stay as they are between others."""
+    heads, page, n = 2, 16, len(lens)
+    cache = gpu.PagedKvCache(n, max(lens), sum(-(-x // page) for x in lens), page, heads, d, quantized=quantized, tracked=True)
+    seqs, models = [cache.add() for _ in lens], [Model(heads, d) for _ in lens]
+    k, v = (synth.normal(1 + i, (n, heads, max(lens), d), stream=i) for i in range(2))
+    cache.append(seqs, _t(gpu, k), _t(gpu, v), lens)
+    w = np.abs(synth.normal(5, (n, heads, max(lens))))
+    cache.addWeights(seqs, _t(gpu, w))
+    cache.evict(seqs, budget, recent)
+    for i, m in enumerate(models):
+        m.append(k[i, :, :lens[i]], v[i, :, :lens[i]], quantized)
+        m.w = [w[i, h, :lens[i]].astype(np.float64) for h in range(heads)]
+        m.evict(budget, recent)
+        got = _check_contents(gpu, cache, seqs[i], m, True)
+        assert np.array_equal(got, np.stack(m.w).astype(np.float32))
