@@ -173,6 +173,8 @@ def prepare(case, seed):
         b, t, hq, hk = case["batch"], case["seq"], case["q_heads"], case["kv_heads"]
         s["q"] = s["qkv"][:, :, :hq].permute(0, 2, 1, 3)
         s["k"] = s["qkv"][:, :, hq:hq + hk].permute(0, 2, 1, 3)
+        if own:
+            torch.cuda.synchronize()  # the framework's stream does not wait for torch's, which makes the inputs
         return s
     n, page = case["seqs"], case["page"]
     lens = {"step": lambda: _lengths(case), "prompt": lambda: [0] * n, "evict": lambda: [case["budget"]] * n}[case["op"]]()
@@ -186,6 +188,9 @@ def prepare(case, seed):
 
 
 def run(state):
+    """One pass.  With ``own`` the outputs are unfinished work on the framework's stream, which torch's does not wait for, nor
+    the other way round: wait for the whole device (torch.cuda.synchronize) before torch reads them, and again after it has
+    read them before they are dropped or the next pass starts, since their memory goes back to an allocator at once."""
     op = state["case"]["op"]
     if op == "rotate":
         return _own_rotate(state) if own else _plain_rotate(state)
