@@ -44,5 +44,25 @@ __device__ __forceinline__ float lanes_max(float v) {
     if (W >= 64) { swap32(v, a, b); v = fmaxf(a, b); }
     return v;
 }
+// The same of the bits of floats that are not negative, which order as the floats do, infinity above them and every NaN
+// above infinity: a maximum that a NaN does not drop out of.
+template <int CTRL>
+__device__ __forceinline__ uint32_t bits_move(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true); }
+template <int W>
+__device__ __forceinline__ uint32_t lanes_max_bits(uint32_t v) {
+    if (W >= 2) v = max(v, bits_move<0xB1>(v));
+    if (W >= 4) v = max(v, bits_move<0x4E>(v));
+    if (W >= 8) v = max(v, bits_move<0x141>(v));
+    if (W >= 16) v = max(v, bits_move<0x140>(v));
+    if (W >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(r[0], r[1]);
+    }
+    if (W >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max(r[0], r[1]);
+    }
+    return v;
+}
 
 }  // namespace mni

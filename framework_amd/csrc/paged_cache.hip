@@ -41,7 +41,9 @@ __global__ __launch_bounds__(TPB) void paged_fork_kernel(const PagedPool p, int 
 // ---- append --------------------------------------------------------------------------------------------------------
 // A group of LPR lanes stores one key row and its value row.  int8: scale = max(max|x| * (1 / 127), 1e-8), codes
 // round(x * (1 / scale)), halves away from zero: a stored value is at most half a scale off, and no code leaves -127 .. 127
-// (the largest is 127 to three roundings).  (The contiguous cache divides by 127; the two scales differ by one rounding.)
+// (the largest is 127 to three roundings).  A row that holds an infinity or a NaN gets that for its scale and codes of 0, so
+// that all of it reads as NaN, in attention too; the maximum is taken of the bits, where a float maximum would lose the NaN.
+// (The contiguous cache divides by 127; the two scales differ by one rounding.)
 // VEC: 4 values per lane, else one value per lane and turn.  Bound by bandwidth: 134 MB of fp32 rows read and written in 46
 // us (5.8 TB/s, the rate of a large copy), 31 MB stored as 8 MB of int8 rows in 9.5.
 template <bool VEC>
@@ -72,12 +74,14 @@ struct AppendRow {
             }
             return;
         }
-        float mx = 0.f;
+        auto bits = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };  // of |v|
+        uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < N; ++j) mx = fmaxf(mx, fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))));
-        mx = lanes_max<LPR>(mx);
-        float scale = mx * (1.0f / 127.0f);
-        if (!(scale > 1e-8f)) scale = 1e-8f;
+        for (int j = 0; j < N; ++j) top = max(top, max(max(bits(x[j].x), bits(x[j].y)), max(bits(x[j].z), bits(x[j].w))));
+        top = lanes_max_bits<LPR>(top);
+        const bool finite = top < 0x7f800000u;
+        float scale = __uint_as_float(top) * (1.0f / 127.0f);
+        if (scale < 1e-8f) scale = 1e-8f;  // (a NaN stays)
         const float inv = 1.0f / scale;
         // halves away from zero: the whole part of y and, towards its sign, the largest value below a half (what round() gives
         // for every |y| up to 128; the product is rounded before the sum, which a fused multiply-add would not do)
@@ -90,12 +94,13 @@ struct AppendRow {
         if (VEC) {
             if (4 * l < d)
                 *reinterpret_cast<uint32_t *>(dst + 4 * l) =
-                    __builtin_amdgcn_perm((uint32_t)code(x[0].w), (uint32_t)code(x[0].z), 0x04000c0c) |
-                    __builtin_amdgcn_perm((uint32_t)code(x[0].y), (uint32_t)code(x[0].x), 0x0c0c0400);
+                    finite ? __builtin_amdgcn_perm((uint32_t)code(x[0].w), (uint32_t)code(x[0].z), 0x04000c0c) |
+                                 __builtin_amdgcn_perm((uint32_t)code(x[0].y), (uint32_t)code(x[0].x), 0x0c0c0400)
+                           : 0u;
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                if (l + 64 * j < d) dst[l + 64 * j] = (signed char)code(x[j].x);
+                if (l + 64 * j < d) dst[l + 64 * j] = (signed char)(finite ? code(x[j].x) : 0);
         }
         if (l == 0) scales[row] = scale;
     }
