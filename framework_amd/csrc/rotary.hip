@@ -378,11 +378,14 @@ int k_qk_norm_rope_backward(const mni_rope_desc &d) {
     RopeArgs a;
     MNI_TRY(rope_args(d, true, &a));
     MNI_TRY(ensure_init());
-    const bool empty = a.tokens == 0;
-    for (const mni_rope_heads *o : {&d.q, &d.k})
-        if (empty && o->heads && o->grad && o->dgamma) MNI_TRY(k_fill(o->dgamma, 0.0f, a.d));
+    bool any = false;  // rows that a gradient comes from
+    for (const mni_rope_heads *o : {&d.q, &d.k}) {
+        if (!o->grad) continue;
+        if (a.tokens > 0 && o->heads > 0) any = true;
+        else if (o->dgamma) MNI_TRY(k_fill(o->dgamma, 0.0f, a.d));  // a sum over no rows
+    }
+    if (!any) return MNI_OK;
     const int64_t heads = d.q.heads > d.k.heads ? d.q.heads : d.k.heads;
-    if (empty || heads == 0 || (!d.q.grad && !d.k.grad)) return MNI_OK;
     const bool pieces = rope_in_pieces(d, true);
     const int lpr = !pieces ? 64 : a.d <= 32 ? 4 : a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32;
     int64_t blocks = ((int64_t)a.tokens * heads + ROPE_TPB / lpr - 1) / (ROPE_TPB / lpr);

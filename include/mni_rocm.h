@@ -287,7 +287,8 @@ typedef struct {
 } mni_rope_desc;
 int mni_rocm_qk_norm_rope(const mni_rope_desc *desc);
 /* Its backward.  With dz the gradient rotated back: dx = r dz g - x r^3 mean(dz g x) and dgamma = the sum over all
- * rows of dz x r, each taken in a fixed order (the same bits every time).  `out` is not read. */
+ * rows of dz x r, each taken in a fixed order (the same bits every time): zeros where there are no rows.  `out` is not
+ * read; an operand without `grad` is left out. */
 int mni_rocm_qk_norm_rope_backward(const mni_rope_desc *desc);
 
 /* ------------------------------------------------------------------------- *
