@@ -198,6 +198,8 @@ void dev_alloc_stats(uint64_t *requests, uint64_t *driver_allocations, uint64_t 
         hipLaunchKernelGGL(__VA_ARGS__); \
     } while (0)
 int check_launch(const char *what);  // hipGetLastError after a kernel launch
+// HIP takes fewer than 2^32 threads along a grid's axis: the workgroups of `threads` threads that one launch may have.
+constexpr int64_t most_blocks(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
 
 // gemm.hip
 int sgemm(const mni_gemm_desc &d);

@@ -118,8 +118,8 @@ __device__ __forceinline__ int page_of(const PagedPool &p, const PagedPrompt &a,
 // A row of keys and values per group of LPR lanes.  (Four rows a group, all asked for before the first is stored: 68
 // against 46 us on 134 MB of fp32 rows, 13 against 10 on 29 MB of them stored as int8.)
 template <bool Q8, bool VEC, int LPR, class Batch>
-__global__ __launch_bounds__(TPB) void paged_append_kernel(const PagedPool p, const PagedNew in, const Batch a) {
-    const uint32_t idx = blockIdx.x * (TPB / LPR) + threadIdx.x / LPR;
+__global__ __launch_bounds__(TPB) void paged_append_kernel(const PagedPool p, const PagedNew in, const Batch a, uint32_t first) {
+    const uint32_t idx = (first + blockIdx.x) * (TPB / LPR) + threadIdx.x / LPR;  // (at most 2^31 rows and a workgroup's)
     const uint32_t ih = idx / (uint32_t)in.tokens, t = idx - ih * in.tokens;
     const uint32_t i = ih / (uint32_t)p.heads, h = ih - i * p.heads;
     if (i >= (uint32_t)a.n || t >= (uint32_t)a.count[i]) return;  // (whole groups leave)
@@ -357,8 +357,11 @@ __global__ __launch_bounds__(TPB) void paged_move_kernel(const EvictArgs a) {
 
 template <bool Q8, bool VEC, int LPR, class Batch>
 void launch_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
-    const uint32_t rows = (uint32_t)a.n * p.heads * in.tokens;
-    MNI_KERNEL_LAUNCH((paged_append_kernel<Q8, VEC, LPR, Batch>), dim3((rows + TPB / LPR - 1) / (TPB / LPR)), dim3(TPB), 0, ctx().stream, p, in, a);
+    const int64_t rows = (int64_t)a.n * p.heads * in.tokens, blocks = (rows + TPB / LPR - 1) / (TPB / LPR);
+    for (int64_t first = 0; first < blocks; first += most_blocks(TPB)) {
+        const int64_t some = blocks - first < most_blocks(TPB) ? blocks - first : most_blocks(TPB);
+        MNI_KERNEL_LAUNCH((paged_append_kernel<Q8, VEC, LPR, Batch>), dim3((unsigned)some), dim3(TPB), 0, ctx().stream, p, in, a, (uint32_t)first);
+    }
 }
 template <class Batch>
 int paged_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
