@@ -23,6 +23,7 @@ struct RopeArgs {
     uint32_t tokens;
     float *part;  // backward: [2][ROPE_BWD_GROUPS][head_dim] partial sums of dgamma
     uint32_t seq, chunks;
+    uint32_t first;  // forward: workgroups of the launches before
     int d, rot, interleaved;
     float eps, inv_d;
     double turns[ROPE_MAX_DIM / 2];  // theta^(-2i / rot) / (2 pi): turns per position of pair i
@@ -99,7 +100,7 @@ __device__ __forceinline__ int64_t rope_out(const mni_rope_heads &o, const RopeA
 // rows, and those are all asked for before.  (HPG is 4 from 65536 rows on, where there are groups enough for it; below, 1.)
 template <int LPR, int HPG>
 __global__ __launch_bounds__(ROPE_TPB) void rope_forward_kernel(const RopeArgs a) {
-    const uint32_t item = blockIdx.x * (ROPE_TPB / LPR) + threadIdx.x / LPR;
+    const uint32_t item = (a.first + blockIdx.x) * (ROPE_TPB / LPR) + threadIdx.x / LPR;
     const uint32_t token = item / a.chunks;
     const int chunk = (int)(item - token * a.chunks);
     if (token >= a.tokens) return;  // (whole groups leave: nothing below crosses a group)
@@ -220,7 +221,7 @@ __device__ __forceinline__ void rope_sincos(const RopeArgs &a, uint32_t token, i
 }
 __global__ __launch_bounds__(ROPE_TPB) void rope_forward_any_kernel(const RopeArgs a) {
     const int heads = (int)(a.q.heads + a.k.heads), lane = threadIdx.x & 63;
-    const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t row = (a.first + blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (row >= a.tokens * heads) return;
     const uint32_t token = row / heads;
     int h = (int)(row - token * heads);
@@ -334,6 +335,7 @@ int rope_args(const mni_rope_desc &d, bool backward, RopeArgs *a) {
     a->rot = (int)d.rotary_dims;
     a->interleaved = d.interleaved != 0;
     a->chunks = 1;
+    a->first = 0;
     a->eps = (float)d.eps;
     a->inv_d = 1.0f / (float)d.head_dim;
     // The last plan's frequencies are kept (a model has one): 64 powers cost as long as a launch.
@@ -347,14 +349,23 @@ int rope_args(const mni_rope_desc &d, bool backward, RopeArgs *a) {
     memcpy(a->turns, turns, sizeof turns);
     return MNI_OK;
 }
+// `blocks` workgroups, in as many launches as grids are needed for them.
+template <class K>
+void rope_launch(K kernel, RopeArgs &a, int64_t blocks) {
+    for (int64_t first = 0; first < blocks; first += most_blocks(ROPE_TPB)) {
+        a.first = (uint32_t)first;
+        const int64_t some = blocks - first < most_blocks(ROPE_TPB) ? blocks - first : most_blocks(ROPE_TPB);
+        MNI_KERNEL_LAUNCH(kernel, dim3((unsigned)some), dim3(ROPE_TPB), 0, ctx().stream, a);
+    }
+}
 template <int LPR>
 void rope_launch_forward(RopeArgs &a) {
     const int64_t heads = a.q.heads + a.k.heads;
     const int per_group = a.tokens * heads >= 65536 ? 4 : 1;
     a.chunks = (uint32_t)((heads + per_group - 1) / per_group);
     const int64_t blocks = ((int64_t)a.tokens * a.chunks + ROPE_TPB / LPR - 1) / (ROPE_TPB / LPR);
-    if (per_group == 4) MNI_KERNEL_LAUNCH((rope_forward_kernel<LPR, 4>), dim3((unsigned)blocks), dim3(ROPE_TPB), 0, ctx().stream, a);
-    else MNI_KERNEL_LAUNCH((rope_forward_kernel<LPR, 1>), dim3((unsigned)blocks), dim3(ROPE_TPB), 0, ctx().stream, a);
+    if (per_group == 4) rope_launch(rope_forward_kernel<LPR, 4>, a, blocks);
+    else rope_launch(rope_forward_kernel<LPR, 1>, a, blocks);
 }
 
 }  // namespace
@@ -365,8 +376,7 @@ int k_qk_norm_rope(const mni_rope_desc &d) {
     const int64_t rows = (int64_t)a.tokens * (d.q.heads + d.k.heads);
     if (rows == 0) return MNI_OK;
     MNI_TRY(ensure_init());
-    if (!rope_in_pieces(d, false))
-        MNI_KERNEL_LAUNCH(rope_forward_any_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(ROPE_TPB), 0, ctx().stream, a);
+    if (!rope_in_pieces(d, false)) rope_launch(rope_forward_any_kernel, a, (rows + 3) / 4);
     else if (a.d <= 32) rope_launch_forward<4>(a);
     else if (a.d <= 64) rope_launch_forward<8>(a);
     else if (a.d <= 128) rope_launch_forward<16>(a);
