@@ -160,14 +160,14 @@ __global__ __launch_bounds__(TPB) void paged_track_kernel(const PagedPool p, con
 }
 // blockIdx.y: head, blockIdx.z: keys or values; a wavefront per row
 __global__ __launch_bounds__(TPB) void paged_read_kernel(const PagedPool p, int slot, int64_t len, float *__restrict__ k, float *__restrict__ v) {
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= len) return;
-    const int64_t row = row_of(p, p.table[slot * p.max_pages + (t >> p.shift)], blockIdx.y, (int)(t & (p.page - 1)));
     const void *cache = blockIdx.z ? p.v : p.k;
-    float *dst = (blockIdx.z ? v : k) + ((int64_t)blockIdx.y * len + t) * p.d;
-    for (int c = threadIdx.x & 63; c < p.d; c += 64)
-        dst[c] = p.quantized ? (float)((const signed char *)cache)[row * p.d + c] * (blockIdx.z ? p.vscale : p.kscale)[row]
-                             : ((const float *)cache)[row * p.d + c];
+    for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < len; t += (int64_t)gridDim.x * 4) {
+        const int64_t row = row_of(p, p.table[slot * p.max_pages + (t >> p.shift)], blockIdx.y, (int)(t & (p.page - 1)));
+        float *dst = (blockIdx.z ? v : k) + ((int64_t)blockIdx.y * len + t) * p.d;
+        for (int c = threadIdx.x & 63; c < p.d; c += 64)
+            dst[c] = p.quantized ? (float)((const signed char *)cache)[row * p.d + c] * (blockIdx.z ? p.vscale : p.kscale)[row]
+                                 : ((const float *)cache)[row * p.d + c];
+    }
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------------
@@ -350,9 +350,9 @@ __global__ __launch_bounds__(SELECT_TPB) void paged_select_kernel(const EvictArg
 __global__ __launch_bounds__(TPB) void paged_move_kernel(const EvictArgs a) {
     const int i = blockIdx.y / a.p.heads, h = blockIdx.y - i * a.p.heads, lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
     const int32_t *moves = a.moves + (int64_t)blockIdx.y * (2 * (int64_t)a.cap + 1);
-    const int j = blockIdx.x * (TPB >> a.lanes_log2) + (threadIdx.x >> a.lanes_log2);
-    if (j >= moves[0]) return;
-    move_row(a, i, h, moves[1 + j], moves[1 + a.cap + j], lane, lanes);
+    const int rows = TPB >> a.lanes_log2, count = moves[0];
+    for (int j = blockIdx.x * rows + (threadIdx.x >> a.lanes_log2); j < count; j += gridDim.x * rows)  // (once, but in the largest grid)
+        move_row(a, i, h, moves[1 + j], moves[1 + a.cap + j], lane, lanes);
 }
 
 template <bool Q8, bool VEC, int LPR, class Batch>
@@ -417,7 +417,8 @@ int k_paged_track(const PagedPool &p, const PagedSeqs &s, float *weights, int32_
 }
 int k_paged_read(const PagedPool &p, int32_t slot, int64_t len, float *k, float *v) {
     if (len <= 0) return MNI_OK;
-    MNI_KERNEL_LAUNCH(paged_read_kernel, dim3((unsigned)((len + 3) / 4), (unsigned)p.heads, 2), dim3(TPB), 0, ctx().stream, p, (int)slot, len, k, v);
+    const int64_t blocks = (len + 3) / 4;
+    MNI_KERNEL_LAUNCH(paged_read_kernel, dim3((unsigned)(blocks < most_blocks(TPB) ? blocks : most_blocks(TPB)), (unsigned)p.heads, 2), dim3(TPB), 0, ctx().stream, p, (int)slot, len, k, v);
     return check_launch("paged_read");
 }
 int k_paged_evict(const PagedPool &p, const PagedSeqs &s, const int32_t *seen, int budget, int recent) {
@@ -450,7 +451,9 @@ int k_paged_evict(const PagedPool &p, const PagedSeqs &s, const int32_t *seen, i
     int rc = check_launch("paged_select");
     if (rc == MNI_OK && !fused) {
         const int per_block = TPB >> a.lanes_log2;
-        MNI_KERNEL_LAUNCH(paged_move_kernel, dim3((unsigned)((a.cap + per_block - 1) / per_block), (unsigned)(s.n * p.heads)), dim3(TPB), 0, ctx().stream, a);
+        const int64_t blocks = (a.cap + per_block - 1) / per_block;
+        MNI_KERNEL_LAUNCH(paged_move_kernel, dim3((unsigned)(blocks < most_blocks(TPB) ? blocks : most_blocks(TPB)), (unsigned)(s.n * p.heads)), dim3(TPB), 0,
+                          ctx().stream, a);
         rc = check_launch("paged_move");
     }
     if (moves) dev_free(moves);

@@ -30,6 +30,39 @@ def test_append_of_more_rows_than_a_grid_holds(gpu, rocm):
     rocm.clear_cache()
 
 
+def test_eviction_and_reading_of_more_rows_than_a_grid_holds(gpu, rocm):
+    budget = (1 << 26) + 9  # a wavefront per row that moves or is read
+    length = 2 * budget
+    cache = gpu.PagedKvCache(1, length, -(-length // 1024), 1024, 1, 1, quantized=False, tracked=True)
+    s = cache.add()
+    k = _values(length)
+    for first in range(0, length, 1 << 24):
+        t = gpu.Tensor.fromFloat32(k[first:first + (1 << 24)], [1, 1, min(1 << 24, length - first), 1])
+        cache.append([s], t, t)
+        t.free()
+
+    def rows(want):
+        for got in cache.read(s):
+            assert np.array_equal(got.numpy().reshape(-1), want)
+            got.free()
+
+    rows(k)
+    w = np.zeros((1, 1, length), np.float32)
+    w[0, 0, budget:] = 1.0  # every row behind the budget takes a place below it, in order
+    t = gpu.Tensor.fromFloat32(w, list(w.shape))
+    cache.addWeights([s], t)
+    t.free()
+    cache.evict([s], budget)
+    assert cache.length(s) == budget
+    rows(k[budget:])
+    weights, positions = cache.track([s])
+    assert (weights.numpy() == 1).all()
+    assert np.array_equal(gpu.native.intBufferToHost(positions), np.arange(budget, length, dtype=np.int32))
+    cache.free()
+    gpu.native.resetEngine()
+    rocm.clear_cache()
+
+
 def test_rotation_of_more_rows_than_a_grid_holds_in_single_values(rocm):
     s = (1 << 26) + 5  # a wavefront per row of one value: the norm alone
     x = _values(s) - np.float32(1 << 23)
