@@ -29,6 +29,7 @@ int set_error(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3
     } while (0)
 
 // ---- device context --------------------------------------------------------
+constexpr int64_t MNI_GRID_THREADS = ((int64_t)1 << 32) - 1;
 struct DeviceCtx {
     bool ready = false;
     int device = 0;
@@ -76,6 +77,8 @@ struct DeviceCtx {
     size_t scratch_bytes = 0;
     // Kernels launched since the library was loaded (bookkeeping for latency-bound steps).
     uint64_t launches = 0;
+    // Threads along an axis of a grid that most_blocks() goes by (tests lower it).
+    int64_t grid_threads = MNI_GRID_THREADS;
     // Device address and size of the library's static workspace (see device.hip).
     float *noalloc_scratch = nullptr;
     size_t noalloc_scratch_bytes = 0;
@@ -198,8 +201,9 @@ void dev_alloc_stats(uint64_t *requests, uint64_t *driver_allocations, uint64_t 
         hipLaunchKernelGGL(__VA_ARGS__); \
     } while (0)
 int check_launch(const char *what);  // hipGetLastError after a kernel launch
-// HIP takes fewer than 2^32 threads along a grid's axis: the workgroups of `threads` threads that one launch may have.
-constexpr int64_t most_blocks(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
+// A grid has fewer than 2^32 threads along an axis (a larger one is cut short without an error): the workgroups of
+// `threads` threads that one launch may have.
+inline int64_t most_blocks(int threads) { return ctx().grid_threads / threads; }
 
 // gemm.hip
 int sgemm(const mni_gemm_desc &d);

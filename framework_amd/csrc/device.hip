@@ -452,6 +452,13 @@ int mni_rocm_test_raise_device_status(unsigned code) {
     return MNI_OK;
 }
 
+int mni_rocm_test_grid_threads(int64_t threads) {
+    MNI_API_GUARD;
+    if (threads != 0 && (threads < 4096 || threads > MNI_GRID_THREADS)) return set_error(MNI_ERR_INVALID, "test_grid_threads: %lld", (long long)threads);
+    ctx().grid_threads = threads ? threads : MNI_GRID_THREADS;
+    return MNI_OK;
+}
+
 int mni_rocm_event_create(void **event) {
     MNI_API_GUARD;
     MNI_TRY(ensure_init());

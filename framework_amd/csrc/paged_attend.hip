@@ -902,6 +902,18 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
         }
     }
     a.first[PAGED_BATCH] = INT_MAX;
+    const int64_t joins = (int64_t)s.n * q_heads * ((p.d + 31) / 32), strips = (longest + 4 * TPB - 1) / (4 * TPB);
+    const int64_t tail = joins + (accumulate ? s.n * p.heads * strips : 0);  // workgroups behind the chunks': see paged_join_kernel
+    if (s.n > 1 && (chunks > most_blocks(TPB) || tail > most_blocks(TPB))) {  // (one sequence alone outgrows the memory before a grid)
+        for (int from : {0, s.n / 2}) {
+            PagedSeqs half;
+            half.n = from ? s.n - from : s.n / 2;
+            for (int i = 0; i < half.n; ++i) { half.slot[i] = s.slot[from + i]; half.len[i] = s.len[from + i]; }
+            const int64_t at = (int64_t)from * q_heads * p.d;
+            MNI_TRY(k_paged_attend(p, half, q + at, out + at, q_heads, scale, accumulate));
+        }
+        return MNI_OK;
+    }
     void *part = nullptr, *ml = nullptr, *scores = nullptr;
     int rc = MNI_OK;
     const bool last = few && !accumulate && most <= LAST_CHUNKS && s.n * rows <= PAGED_TICKETS;
@@ -955,10 +967,9 @@ int k_paged_attend(const PagedPool &p, const PagedSeqs &s, const float *q, float
         rc = check_launch("paged_attend");
     }
     if (rc == MNI_OK && a.part && !last) {
-        const int joins = s.n * q_heads * ((p.d + 31) / 32), tiles = (int)((longest + 4 * TPB - 1) / (4 * TPB));
-        const dim3 grid((unsigned)(joins + (accumulate ? s.n * p.heads * tiles : 0)));
-        if (p.d % 4 == 0) MNI_KERNEL_LAUNCH(paged_join_kernel<4>, grid, dim3(TPB), 0, ctx().stream, a, joins, tiles);
-        else MNI_KERNEL_LAUNCH(paged_join_kernel<1>, grid, dim3(TPB), 0, ctx().stream, a, joins, tiles);
+        const dim3 grid((unsigned)tail);
+        if (p.d % 4 == 0) MNI_KERNEL_LAUNCH(paged_join_kernel<4>, grid, dim3(TPB), 0, ctx().stream, a, (int)joins, (int)strips);
+        else MNI_KERNEL_LAUNCH(paged_join_kernel<1>, grid, dim3(TPB), 0, ctx().stream, a, (int)joins, (int)strips);
         rc = check_launch("paged_join");
     }
     if (part) dev_free(part);

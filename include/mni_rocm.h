@@ -519,6 +519,11 @@ void *mni_rocm_int_buffer_ptr(uint32_t id);
  * expired would: the next call that waits for the stream reports it. */
 int mni_rocm_test_raise_device_status(unsigned code);
 
+/* Lowers the number of threads along a grid's axis that calls with more rows
+ * than one grid holds split themselves by (4096 up to 2^32 - 1; 0 restores
+ * it), so that their several launches can be tested on small sizes. */
+int mni_rocm_test_grid_threads(int64_t threads);
+
 /* Kernels launched by the library since it was loaded (copies not counted):
  * what a latency-bound training step is made of. */
 uint64_t mni_rocm_launch_count(void);
