@@ -79,6 +79,7 @@ struct DeviceCtx {
     uint64_t launches = 0;
     // Threads along an axis of a grid that most_blocks() goes by (tests lower it).
     int64_t grid_threads = MNI_GRID_THREADS;
+    int64_t paged_launch_fails_in = 0;  // tests: the launch of a paged cache's change that is reported as failed (0: none)
     // Device address and size of the library's static workspace (see device.hip).
     float *noalloc_scratch = nullptr;
     size_t noalloc_scratch_bytes = 0;

@@ -459,6 +459,13 @@ int mni_rocm_test_grid_threads(int64_t threads) {
     return MNI_OK;
 }
 
+int mni_rocm_test_fail_paged_launch(int64_t n) {
+    MNI_API_GUARD;
+    if (n < 0) return set_error(MNI_ERR_INVALID, "test_fail_paged_launch: %lld", (long long)n);
+    ctx().paged_launch_fails_in = n;
+    return MNI_OK;
+}
+
 int mni_rocm_event_create(void **event) {
     MNI_API_GUARD;
     MNI_TRY(ensure_init());

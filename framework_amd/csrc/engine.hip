@@ -1941,16 +1941,26 @@ static void paged_release(PagedCache &c, PagedSequence &s, int64_t keep) {  // t
     }
 }
 static int64_t paged_entry(const PagedCache &c, uint32_t seq, int64_t page) { return (int64_t)seq * c.pool.max_pages + page; }
+// Makes the copies listed so far.  Where that fails their sequences go back to the pages that they shared.
+static int paged_make_copies(PagedCache &c, PagedCopies &copies) {
+    const int rc = k_paged_copy(c.pool, copies);
+    if (rc != MNI_OK)
+        for (int i = copies.n; i-- > 0;) {
+            c.seqs[copies.at[i] / c.pool.max_pages].pages[copies.at[i] % c.pool.max_pages] = copies.from[i];
+            ++c.holders[copies.from[i]];
+            c.holders[copies.to[i]] = 0;
+            c.free_pages.push_back(copies.to[i]);
+        }
+    copies.n = 0;
+    return rc;
+}
 // Own copies of the pages [from, to) of a sequence that others hold too.  The caller has made sure of enough pages.
 static int paged_unshare(PagedCache &c, uint32_t seq, int64_t from, int64_t to, PagedCopies &copies) {
     PagedSequence &s = c.seqs[seq];
     for (int64_t j = from; j < to; ++j) {
         const int32_t page = s.pages[j];
         if (c.holders[page] <= 1) continue;
-        if (copies.n == PAGED_COPIES) {
-            MNI_TRY(k_paged_copy(c.pool, copies));
-            copies.n = 0;
-        }
+        if (copies.n == PAGED_COPIES) MNI_TRY(paged_make_copies(c, copies));
         copies.at[copies.n] = paged_entry(c, seq, j);
         copies.from[copies.n] = page;
         --c.holders[page];
@@ -2032,6 +2042,7 @@ static uint32_t paged_add(PagedCache &c) {
 }
 static uint32_t paged_fork(PagedCache &c, uint32_t from) {
     if (!paged_seq(c, from)) return MNI_BAD_ID;
+    PagedSequence copy = c.seqs[from];  // (what may run out of memory comes first)
     const uint32_t seq = paged_add(c);
     if (seq == MNI_BAD_ID) return MNI_BAD_ID;
     if (k_paged_fork(c.pool, (int32_t)from, (int32_t)seq, c.seqs[from].len) != MNI_OK) {
@@ -2039,7 +2050,7 @@ static uint32_t paged_fork(PagedCache &c, uint32_t from) {
         c.free_seqs.push_back(seq);
         return MNI_BAD_ID;
     }
-    c.seqs[seq] = c.seqs[from];
+    c.seqs[seq] = std::move(copy);
     for (int32_t page : c.seqs[seq].pages) ++c.holders[page];
     return seq;
 }
@@ -2048,6 +2059,64 @@ static int paged_write_table(PagedCache &c, uint32_t seq, int64_t had) {
     const std::vector<int32_t> &pages = c.seqs[seq].pages;
     for (size_t j = (size_t)had; j < pages.size(); j += DeviceCtx::STAGE_BYTES / 4)
         MNI_TRY(upload_small(c.pool.table + paged_entry(c, seq, (int64_t)j), pages.data() + j, std::min<size_t>(DeviceCtx::STAGE_BYTES / 4, pages.size() - j) * 4));
+    return MNI_OK;
+}
+// The launches of an append: rows of k and v go behind the ends of their sequences, whose lengths grow launch by launch.
+// `had`: pages that each sequence had before.
+static int paged_append_rows(PagedCache &c, const uint32_t *seqs, size_t n, const int64_t *counts, PagedNew in, const float *k, const float *v,
+                             const std::vector<int64_t> &had) {
+    const int64_t tokens = in.tokens;
+    auto inputs = [&](size_t first) {
+        in.k = k + (int64_t)first * in.k_seq;
+        in.v = v + (int64_t)first * in.v_seq;
+    };
+    auto enter = [&](auto &a, size_t i) {
+        PagedSequence &s = c.seqs[seqs[i]];
+        const int at = a.n++;
+        a.slot[at] = (int32_t)seqs[i];
+        a.len[at] = (int32_t)s.len;
+        a.count[at] = (int32_t)(counts ? counts[i] : tokens);
+        a.seen[at] = (int32_t)s.seen;
+        s.len += a.count[at];
+        s.seen += a.count[at];
+        return at;
+    };
+    if (tokens == 1) {
+        for (size_t first = 0; first < n; first += PagedAppend::MAX) {
+            PagedAppend a;
+            a.n = 0;
+            inputs(first);
+            for (size_t i = first; i < n && a.n < PagedAppend::MAX; ++i) {
+                const int at = enter(a, i);
+                const PagedSequence &s = c.seqs[seqs[i]];
+                a.page[at] = (int64_t)s.pages.size() > had[i] ? s.pages.back() : -1;
+            }
+            MNI_TRY(k_paged_append(c.pool, in, a));
+        }
+        return MNI_OK;
+    }
+    for (size_t first = 0; first < n;) {
+        PagedPrompt a;
+        a.n = 0;
+        inputs(first);
+        int used = 0;
+        for (; first < n && a.n < PagedPrompt::MAX; ++first) {
+            const std::vector<int32_t> &pages = c.seqs[seqs[first]].pages;
+            const int64_t fresh = (int64_t)pages.size() - had[first];
+            if (fresh <= PAGED_PROMPT_PAGES && used + fresh > PAGED_PROMPT_PAGES) break;  // (fits the next launch's)
+            const int at = enter(a, first);
+            a.first[at] = used;
+            a.had[at] = (int32_t)had[first];
+            if (fresh > PAGED_PROMPT_PAGES) {
+                MNI_TRY(paged_write_table(c, seqs[first], had[first]));
+                a.had[at] = INT32_MAX;
+            } else {
+                std::copy(pages.begin() + had[first], pages.end(), a.pages + used);
+                used += (int)fresh;
+            }
+        }
+        MNI_TRY(k_paged_append(c.pool, in, a));
+    }
     return MNI_OK;
 }
 static int paged_append(PagedCache &c, const uint32_t *seqs, size_t n, uint32_t k, uint32_t v, const int64_t *counts) {
@@ -2098,69 +2167,37 @@ static int paged_append(PagedCache &c, const uint32_t *seqs, size_t n, uint32_t 
     in.k_seq = kst[0]; in.k_head = kst[1]; in.k_token = kst[2];
     in.v_seq = vst[0]; in.v_head = vst[1]; in.v_token = vst[2];
     in.tokens = (int)tokens;
+    struct Before { int64_t len, seen; };
+    std::vector<Before> before(n);
+    std::vector<int64_t> had(n);
     PagedCopies copies;
     copies.n = 0;
-    std::vector<int64_t> had(n);
+    for (size_t i = 0; i < n; ++i) {  // (a copy changes nothing of what a sequence holds)
+        const PagedSequence &s = c.seqs[seqs[i]];
+        if ((counts ? counts[i] : tokens) > 0 && (s.len & (p.page - 1)))
+            MNI_TRY(paged_unshare(c, seqs[i], (int64_t)s.pages.size() - 1, (int64_t)s.pages.size(), copies));
+    }
+    MNI_TRY(paged_make_copies(c, copies));
+    for (size_t i = 0; i < n; ++i) {  // room for the page lists, before the first of them grows
+        PagedSequence &s = c.seqs[seqs[i]];
+        const size_t want = (size_t)paged_pages(c, s.len + (counts ? counts[i] : tokens));
+        if (s.pages.capacity() < want) s.pages.reserve(std::max(want, 2 * s.pages.capacity()));
+    }
     for (size_t i = 0; i < n; ++i) {
         PagedSequence &s = c.seqs[seqs[i]];
-        const int64_t count = counts ? counts[i] : tokens;
-        if (count > 0 && (s.len & (p.page - 1))) MNI_TRY(paged_unshare(c, seqs[i], (int64_t)s.pages.size() - 1, (int64_t)s.pages.size(), copies));
+        before[i] = {s.len, s.seen};
         had[i] = (int64_t)s.pages.size();
-        while ((int64_t)s.pages.size() < paged_pages(c, s.len + count)) s.pages.push_back(paged_take(c));
+        while ((int64_t)s.pages.size() < paged_pages(c, s.len + (counts ? counts[i] : tokens))) s.pages.push_back(paged_take(c));
     }
-    MNI_TRY(k_paged_copy(p, copies));
-    auto inputs = [&](size_t first) {
-        in.k = kb->p + (int64_t)first * in.k_seq;
-        in.v = vb->p + (int64_t)first * in.v_seq;
-    };
-    auto enter = [&](auto &a, size_t i) {
-        PagedSequence &s = c.seqs[seqs[i]];
-        const int k = a.n++;
-        a.slot[k] = (int32_t)seqs[i];
-        a.len[k] = (int32_t)s.len;
-        a.count[k] = (int32_t)(counts ? counts[i] : tokens);
-        a.seen[k] = (int32_t)s.seen;
-        s.len += a.count[k];
-        s.seen += a.count[k];
-        return k;
-    };
-    if (tokens == 1) {
-        for (size_t first = 0; first < n; first += PagedAppend::MAX) {
-            PagedAppend a;
-            a.n = 0;
-            inputs(first);
-            for (size_t i = first; i < n && a.n < PagedAppend::MAX; ++i) {
-                const int k = enter(a, i);
-                const PagedSequence &s = c.seqs[seqs[i]];
-                a.page[k] = (int64_t)s.pages.size() > had[i] ? s.pages.back() : -1;
-            }
-            MNI_TRY(k_paged_append(p, in, a));
+    const int rc = paged_append_rows(c, seqs, n, counts, in, kb->p, vb->p, had);
+    if (rc != MNI_OK)  // all lengths go back; what was written lies behind them
+        for (size_t i = n; i-- > 0;) {
+            PagedSequence &s = c.seqs[seqs[i]];
+            s.len = before[i].len;
+            s.seen = before[i].seen;
+            paged_release(c, s, had[i]);
         }
-        return MNI_OK;
-    }
-    for (size_t first = 0; first < n;) {
-        PagedPrompt a;
-        a.n = 0;
-        inputs(first);
-        int used = 0;
-        for (; first < n && a.n < PagedPrompt::MAX; ++first) {
-            const std::vector<int32_t> &pages = c.seqs[seqs[first]].pages;
-            const int64_t fresh = (int64_t)pages.size() - had[first];
-            if (fresh <= PAGED_PROMPT_PAGES && used + fresh > PAGED_PROMPT_PAGES) break;  // (fits the next launch's)
-            const int k = enter(a, first);
-            a.first[k] = used;
-            a.had[k] = (int32_t)had[first];
-            if (fresh > PAGED_PROMPT_PAGES) {
-                MNI_TRY(paged_write_table(c, seqs[first], had[first]));
-                a.had[k] = INT32_MAX;
-            } else {
-                std::copy(pages.begin() + had[first], pages.end(), a.pages + used);
-                used += (int)fresh;
-            }
-        }
-        MNI_TRY(k_paged_append(p, in, a));
-    }
-    return MNI_OK;
+    return rc;
 }
 static int paged_truncate(PagedCache &c, const uint32_t *seqs, size_t n, const int64_t *lens) {
     MNI_TRY(paged_check(c, seqs, n, true, "truncate"));
@@ -2244,18 +2281,18 @@ static int paged_evict(PagedCache &c, const uint32_t *seqs, size_t n, int64_t bu
     copies.n = 0;
     for (size_t i = 0; i < n; ++i)
         if (c.seqs[seqs[i]].len > budget) MNI_TRY(paged_unshare(c, seqs[i], 0, keep, copies));
-    MNI_TRY(k_paged_copy(p, copies));
-    for (size_t first = 0; first < n; first += PAGED_BATCH) {
-        const PagedSeqs s = paged_batch(c, seqs, first, n);
+    MNI_TRY(paged_make_copies(c, copies));
+    for (size_t first = 0; first < n; first += PAGED_BATCH) {  // lengths change with the rows, launch by launch
+        const PagedSeqs batch = paged_batch(c, seqs, first, n);
         int32_t seen[PAGED_BATCH];
-        for (int i = 0; i < s.n; ++i) seen[i] = (int32_t)c.seqs[seqs[first + i]].seen;
-        MNI_TRY(k_paged_evict(p, s, seen, (int)std::min<int64_t>(budget, INT32_MAX), (int)std::min<int64_t>(recent, INT32_MAX)));
-    }
-    for (size_t i = n; i-- > 0;) {
-        PagedSequence &s = c.seqs[seqs[i]];
-        if (s.len <= budget) continue;
-        s.len = s.floor = budget;
-        paged_release(c, s, keep);
+        for (int i = 0; i < batch.n; ++i) seen[i] = (int32_t)c.seqs[seqs[first + i]].seen;
+        MNI_TRY(k_paged_evict(p, batch, seen, (int)std::min<int64_t>(budget, INT32_MAX), (int)std::min<int64_t>(recent, INT32_MAX)));
+        for (int i = batch.n; i-- > 0;) {
+            PagedSequence &s = c.seqs[seqs[first + i]];
+            if (s.len <= budget) continue;
+            s.len = s.floor = budget;
+            paged_release(c, s, keep);
+        }
     }
     return MNI_OK;
 }

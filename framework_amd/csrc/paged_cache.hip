@@ -355,6 +355,11 @@ __global__ __launch_bounds__(TPB) void paged_move_kernel(const EvictArgs a) {
         move_row(a, i, h, moves[1 + j], moves[1 + a.cap + j], lane, lanes);
 }
 
+int launch_allowed(const char *what) {  // (see mni_rocm_test_fail_paged_launch)
+    int64_t &left = ctx().paged_launch_fails_in;
+    if (left > 0 && --left == 0) return set_error(MNI_ERR_HIP, "launch of %s failed: a test asked for it", what);
+    return MNI_OK;
+}
 template <bool Q8, bool VEC, int LPR, class Batch>
 void launch_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
     const int64_t rows = (int64_t)a.n * p.heads * in.tokens, blocks = (rows + TPB / LPR - 1) / (TPB / LPR);
@@ -366,6 +371,7 @@ void launch_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
 template <class Batch>
 int paged_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
     if (a.n <= 0 || in.tokens <= 0) return MNI_OK;
+    MNI_TRY(launch_allowed("paged_append"));
     const bool vec = p.d % 4 == 0 && (((uintptr_t)in.k | (uintptr_t)in.v) & 15) == 0 &&
                      ((in.k_seq | in.k_head | in.k_token | in.v_seq | in.v_head | in.v_token) & 3) == 0;
     if (!vec) {
@@ -387,6 +393,7 @@ int paged_append(const PagedPool &p, const PagedNew &in, const Batch &a) {
 
 int k_paged_copy(const PagedPool &p, const PagedCopies &c) {
     if (c.n <= 0) return MNI_OK;
+    MNI_TRY(launch_allowed("paged_copy"));
     const int64_t bytes = (int64_t)p.heads * p.page * p.d * (p.quantized ? 1 : 4), parts = (bytes + 16383) / 16384;
     MNI_KERNEL_LAUNCH(paged_copy_kernel, dim3((unsigned)c.n, p.quantized ? 4 : 2, (unsigned)(parts < 1024 ? parts : 1024)), dim3(TPB), 0, ctx().stream, p, c);
     return check_launch("paged_copy");
@@ -436,6 +443,7 @@ int k_paged_evict(const PagedPool &p, const PagedSeqs &s, const int32_t *seen, i
     }
     const int64_t behind = longest - budget;
     if (s.n <= 0 || behind <= 0 || budget <= 0) return MNI_OK;
+    MNI_TRY(launch_allowed("paged_select"));
     a.cap = (int)(behind < budget ? behind : budget);  // at most so many rows change place
     const int bytes = p.d * (p.quantized ? 1 : 4);
     a.lanes_log2 = 0;

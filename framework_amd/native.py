@@ -103,6 +103,7 @@ SIGNATURES = {
     "mni_rocm_qk_norm_rope": (C.c_int, [C.c_void_p]),  # a RopeDesc, packed
     "mni_rocm_qk_norm_rope_backward": (C.c_int, [C.c_void_p]),
     "mni_rocm_test_grid_threads": (C.c_int, [C.c_int64]),
+    "mni_rocm_test_fail_paged_launch": (C.c_int, [C.c_int64]),
     "mni_zeros": (C.c_uint32, [_i64p, C.c_int]),
     "mni_ones": (C.c_uint32, [_i64p, C.c_int]),
     "mni_from_float32": (C.c_uint32, [C.c_void_p, C.c_size_t, _i64p, C.c_int]),
@@ -275,6 +276,9 @@ class Rocm:
 
     def test_grid_threads(self, threads):
         self._check(self.lib.mni_rocm_test_grid_threads(threads))
+
+    def test_fail_paged_launch(self, n):
+        self._check(self.lib.mni_rocm_test_fail_paged_launch(n))
 
     def test_raise_device_status(self, code):
         self._check(self.lib.mni_rocm_test_raise_device_status(code))

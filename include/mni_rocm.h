@@ -464,7 +464,7 @@ int mni_qk_norm_rope(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k,
  *   not change it); free_pages: pages that no sequence holds.  < 0 for an unknown id.
  * append: k, v [n, kv_heads, T, head_dim] (views welcome): sequence seqs[i] takes its first counts[i] <= T tokens, or
  *   all T where counts is NULL.  A sequence may not occur twice, kv_heads * T may not pass 2^24.  Only rows behind a
- *   sequence's end are written; a call that is refused has changed nothing.
+ *   sequence's end are written; a call that is refused or fails has changed no sequence's rows or length.
  * truncate: back to lens[i] rows, the tokens appended last leave first (rejected drafts).  Of a sequence that has
  *   been evicted only tokens appended since then can leave this way.
  * attend: q [n, heads, 1, head_dim] (or [n * heads, 1, head_dim]) attends over everything seqs[i] holds: softmax(scale
@@ -476,7 +476,8 @@ int mni_qk_norm_rope(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k,
  *   tokens stay, then those of the largest weight, equal weights by the earlier position (a NaN counts as the
  *   largest).  A row that stays below the budget keeps its place; the freed places take the surviving rows behind the
  *   budget, in order, with their weights and positions.  Pages behind the budget are freed; pages shared with a fork
- *   are copied first.
+ *   are copied first.  A call that is refused has changed nothing; one that fails on the device has cut each sequence
+ *   wholly or not at all (its length tells).
  * track: the weights, as a tensor [n, kv_heads, longest], and the positions, as an int buffer of as many values, of
  *   every row in the order held; 0 and -1 behind a sequence's end.
  * read: keys and values of one sequence in the order held, [kv_heads, len, head_dim] (int8 rows as the values they
@@ -523,6 +524,11 @@ int mni_rocm_test_raise_device_status(unsigned code);
  * than one grid holds split themselves by (4096 up to 2^32 - 1; 0 restores
  * it), so that their several launches can be tested on small sizes. */
 int mni_rocm_test_grid_threads(int64_t threads);
+
+/* The n-th launch from now on of a paged cache's append, page copy or
+ * eviction is not made and reported as failed (0: none), so that tests can
+ * see what such a failure leaves. */
+int mni_rocm_test_fail_paged_launch(int64_t n);
 
 /* Kernels launched by the library since it was loaded (copies not counted):
  * what a latency-bound training step is made of. */
