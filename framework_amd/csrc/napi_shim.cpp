@@ -10,6 +10,7 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include <new>
 #include <vector>
 
 #include "../../include/mni_rocm.h"
@@ -312,132 +313,191 @@ bool is_given(napi_env env, napi_value v) {  // neither undefined nor null
     napi_valuetype t;
     return napi_typeof(env, v, &t) == napi_ok && t != napi_undefined && t != napi_null;
 }
+// Arguments that have to be what they are said to be: an id or a length that is silently taken for 0 would name a sequence
+// that the caller did not mean.  What is not throws, and `ok` is false from then on.
+struct Strict {
+    napi_env env;
+    bool ok = true;
+    void refuse(const char *what) {
+        if (ok) napi_throw_error(env, nullptr, what);
+        ok = false;
+    }
+    double number(napi_value v, const char *what) {
+        double x = 0;
+        if (napi_get_value_double(env, v, &x) != napi_ok) refuse(what);
+        return x;
+    }
+    bool whole(double x, bool id) {  // ids of 32 bits (the last one names nothing), else what a double holds exactly
+        return x >= (id ? 0.0 : -9007199254740991.0) && x <= (id ? 4294967294.0 : 9007199254740991.0) && x == (double)(int64_t)x;
+    }
+    uint32_t id(napi_value v) {
+        const char *what = "an id, a whole number from 0 up to 2^32 - 2, is wanted";
+        const double x = number(v, what);
+        if (!whole(x, true)) refuse(what);
+        return ok ? (uint32_t)x : 0;
+    }
+    int64_t count(napi_value v) {
+        const char *what = "a whole number is wanted";
+        const double x = number(v, what);
+        if (!whole(x, false)) refuse(what);
+        return ok ? (int64_t)x : 0;
+    }
+    int64_t count_or_zero(napi_value v) { return is_given(env, v) ? count(v) : 0; }
+    // A list of ids (uint32_t) or lengths (int64_t): an array, or a typed array of 32-bit integers or doubles.
+    template <class V>
+    std::vector<V> list(napi_value v, const char *what) {
+        constexpr bool ids = sizeof(V) == 4;
+        std::vector<V> out;
+        if (!ok) return out;
+        auto take = [&](double x) {
+            if (!whole(x, ids)) return refuse(ids ? "every id must be a whole number from 0 up to 2^32 - 2" : "every length must be a whole number");
+            out.push_back((V)x);
+        };
+        try {
+            bool is = false;
+            if (napi_is_array(env, v, &is) == napi_ok && is) {
+                uint32_t n = 0;
+                napi_get_array_length(env, v, &n);
+                for (uint32_t i = 0; i < n && ok; ++i) {
+                    napi_value e;
+                    double x = -0.5;  // (no whole number)
+                    if (napi_get_element(env, v, i, &e) != napi_ok || napi_get_value_double(env, e, &x) != napi_ok) x = -0.5;
+                    take(x);
+                }
+                return out;
+            }
+            napi_typedarray_type type;
+            size_t n = 0;
+            void *data = nullptr;
+            if (napi_is_typedarray(env, v, &is) == napi_ok && is && napi_get_typedarray_info(env, v, &type, &n, &data, nullptr, nullptr) == napi_ok &&
+                (type == napi_uint32_array || type == napi_int32_array || type == napi_float64_array)) {
+                for (size_t i = 0; i < n && ok; ++i)
+                    take(type == napi_uint32_array ? ((const uint32_t *)data)[i] : type == napi_int32_array ? ((const int32_t *)data)[i] : ((const double *)data)[i]);
+                return out;
+            }
+        } catch (const std::bad_alloc &) {
+            refuse("out of host memory for a list");
+            return out;
+        }
+        refuse(what);
+        return out;
+    }
+    std::vector<uint32_t> seqs(napi_value v) { return list<uint32_t>(v, "paged cache: an array of sequence ids is wanted"); }
+};
 napi_value QkNormRope(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    uint32_t out[2] = {0, 0};
-    const int rc = mni_qk_norm_rope(get_u32(env, a.v[0]), get_u32(env, a.v[1]), get_u32(env, a.v[2]), get_u32(env, a.v[3]),
-                                    is_given(env, a.v[4]) ? get_u32(env, a.v[4]) : MNI_BAD_ID, get_i64(env, a.v[5]), get_i64(env, a.v[6]),
-                                    get_bool(env, a.v[7]) ? 1 : 0, get_f64(env, a.v[8]), get_f64(env, a.v[9]), out);
-    return ret_ids(env, rc, out[0], out[1]);
+    Strict s{env};
+    uint32_t in[4], out[2] = {0, 0};
+    for (int i = 0; i < 4; ++i) in[i] = s.id(a.v[i]);
+    const uint32_t positions = is_given(env, a.v[4]) ? s.id(a.v[4]) : MNI_BAD_ID;
+    const int64_t offset = s.count_or_zero(a.v[5]), rotary = s.count(a.v[6]);
+    const double theta = s.number(a.v[8], "qkNormRope: theta must be a number"), eps = s.number(a.v[9], "qkNormRope: eps must be a number");
+    if (!s.ok) return nullptr;
+    return ret_ids(env, mni_qk_norm_rope(in[0], in[1], in[2], in[3], positions, offset, rotary, get_bool(env, a.v[7]) ? 1 : 0, theta, eps, out), out[0], out[1]);
 }
 napi_value PagedCacheCreate(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    return ret_id(env, mni_paged_cache_create(get_i64(env, a.v[0]), get_i64(env, a.v[1]), get_i64(env, a.v[2]), get_i64(env, a.v[3]), get_i64(env, a.v[4]),
-                                              get_i64(env, a.v[5]), get_bool(env, a.v[6]) ? 1 : 0, get_bool(env, a.v[7]) ? 1 : 0));
+    Strict s{env};
+    int64_t n[6];
+    for (int i = 0; i < 6; ++i) n[i] = s.count(a.v[i]);
+    if (!s.ok) return nullptr;
+    return ret_id(env, mni_paged_cache_create(n[0], n[1], n[2], n[3], n[4], n[5], get_bool(env, a.v[6]) ? 1 : 0, get_bool(env, a.v[7]) ? 1 : 0));
 }
 napi_value PagedCacheFree(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    mni_paged_cache_free(get_u32(env, a.v[0]));
+    Strict s{env};
+    const uint32_t cache = s.id(a.v[0]);
+    if (!s.ok) return nullptr;
+    mni_paged_cache_free(cache);
     return undefined(env);
 }
 napi_value ret_count(napi_env env, int64_t n) { return n < 0 ? throw_last(env) : make_f64(env, (double)n); }
-napi_value PagedCacheFreePages(napi_env env, napi_callback_info info) {
-    Args a(env, info);
-    return ret_count(env, mni_paged_cache_free_pages(get_u32(env, a.v[0])));
-}
-napi_value PagedCacheAdd(napi_env env, napi_callback_info info) {
-    Args a(env, info);
-    return ret_id(env, mni_paged_cache_add(get_u32(env, a.v[0])));
-}
-napi_value PagedCacheFork(napi_env env, napi_callback_info info) {
-    Args a(env, info);
-    return ret_id(env, mni_paged_cache_fork(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
-}
-napi_value PagedCacheDrop(napi_env env, napi_callback_info info) {
-    Args a(env, info);
-    return ret_rc(env, mni_paged_cache_drop(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
-}
-napi_value PagedCacheLen(napi_env env, napi_callback_info info) {
-    Args a(env, info);
-    return ret_count(env, mni_paged_cache_len(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
-}
-napi_value PagedCacheSeen(napi_env env, napi_callback_info info) {
-    Args a(env, info);
-    return ret_count(env, mni_paged_cache_seen(get_u32(env, a.v[0]), get_u32(env, a.v[1])));
-}
-// A list of ids or lengths: an array, or a typed array of 32-bit integers or doubles.  Anything else throws (false).
-template <class V>
-bool get_list(napi_env env, napi_value v, std::vector<V> *out, const char *what) {
-    bool is = false;
-    if (napi_is_array(env, v, &is) == napi_ok && is) {
-        uint32_t n = 0;
-        napi_get_array_length(env, v, &n);
-        out->resize(n);
-        for (uint32_t i = 0; i < n; ++i) {
-            napi_value e;
-            napi_get_element(env, v, i, &e);
-            (*out)[i] = (V)get_i64(env, e);
-        }
-        return true;
+// NAME(cache), NAME(cache, sequence)
+#define PAGED_CACHE(NAME, FN, RET)                                  \
+    napi_value NAME(napi_env env, napi_callback_info info) {        \
+        Args a(env, info);                                          \
+        Strict s{env};                                              \
+        const uint32_t cache = s.id(a.v[0]);                        \
+        return s.ok ? RET(env, FN(cache)) : nullptr;                \
     }
-    napi_typedarray_type type;
-    size_t n = 0;
-    void *data = nullptr;
-    if (napi_is_typedarray(env, v, &is) == napi_ok && is && napi_get_typedarray_info(env, v, &type, &n, &data, nullptr, nullptr) == napi_ok) {
-        auto copy = [&](auto *from) { out->resize(n); for (size_t i = 0; i < n; ++i) (*out)[i] = (V)from[i]; return true; };
-        if (type == napi_uint32_array) return copy((const uint32_t *)data);
-        if (type == napi_int32_array) return copy((const int32_t *)data);
-        if (type == napi_float64_array) return copy((const double *)data);
+#define PAGED_SEQUENCE(NAME, FN, RET)                               \
+    napi_value NAME(napi_env env, napi_callback_info info) {        \
+        Args a(env, info);                                          \
+        Strict s{env};                                              \
+        const uint32_t cache = s.id(a.v[0]), seq = s.id(a.v[1]);    \
+        return s.ok ? RET(env, FN(cache, seq)) : nullptr;           \
     }
-    napi_throw_error(env, nullptr, what);
-    return false;
-}
-napi_value throw_lengths(napi_env env, const char *what) {
-    napi_throw_error(env, nullptr, what);
-    return nullptr;
-}
-constexpr const char *WANT_SEQS = "paged cache: an array of sequence ids is wanted";
+PAGED_CACHE(PagedCacheFreePages, mni_paged_cache_free_pages, ret_count)
+PAGED_CACHE(PagedCacheAdd, mni_paged_cache_add, ret_id)
+PAGED_SEQUENCE(PagedCacheFork, mni_paged_cache_fork, ret_id)
+PAGED_SEQUENCE(PagedCacheDrop, mni_paged_cache_drop, ret_rc)
+PAGED_SEQUENCE(PagedCacheLen, mni_paged_cache_len, ret_count)
+PAGED_SEQUENCE(PagedCacheSeen, mni_paged_cache_seen, ret_count)
 napi_value PagedCacheAppend(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    std::vector<uint32_t> seqs;
-    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
+    Strict s{env};
+    const std::vector<uint32_t> seqs = s.seqs(a.v[1]);
+    const uint32_t cache = s.id(a.v[0]), k = s.id(a.v[2]), v = s.id(a.v[3]);
     const bool some = is_given(env, a.v[4]);
     std::vector<int64_t> counts;
-    if (some && !get_list(env, a.v[4], &counts, "paged cache append: an array of counts is wanted")) return nullptr;
-    if (some && counts.size() != seqs.size()) return throw_lengths(env, "paged cache append: as many counts as sequences are wanted");
-    return ret_rc(env, mni_paged_cache_append(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2]), get_u32(env, a.v[3]),
-                                              some ? counts.data() : nullptr));
+    if (some) counts = s.list<int64_t>(a.v[4], "paged cache append: an array of counts is wanted");
+    if (some && counts.size() != seqs.size()) s.refuse("paged cache append: as many counts as sequences are wanted");
+    if (!s.ok) return nullptr;
+    return ret_rc(env, mni_paged_cache_append(cache, seqs.data(), seqs.size(), k, v, some ? counts.data() : nullptr));
 }
 napi_value PagedCacheTruncate(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    std::vector<uint32_t> seqs;
-    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
-    std::vector<int64_t> lens;
-    if (!get_list(env, a.v[2], &lens, "paged cache truncate: an array of lengths is wanted")) return nullptr;
-    if (lens.size() != seqs.size()) return throw_lengths(env, "paged cache truncate: as many lengths as sequences are wanted");
-    return ret_rc(env, mni_paged_cache_truncate(get_u32(env, a.v[0]), seqs.data(), seqs.size(), lens.data()));
+    Strict s{env};
+    const std::vector<uint32_t> seqs = s.seqs(a.v[1]);
+    const std::vector<int64_t> lens = s.list<int64_t>(a.v[2], "paged cache truncate: an array of lengths is wanted");
+    const uint32_t cache = s.id(a.v[0]);
+    if (lens.size() != seqs.size()) s.refuse("paged cache truncate: as many lengths as sequences are wanted");
+    if (!s.ok) return nullptr;
+    return ret_rc(env, mni_paged_cache_truncate(cache, seqs.data(), seqs.size(), lens.data()));
 }
 napi_value PagedCacheAttend(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    std::vector<uint32_t> seqs;
-    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
-    return ret_id(env, mni_paged_cache_attend(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2]), get_f64(env, a.v[3]),
-                                              get_bool(env, a.v[4]) ? 1 : 0));
+    Strict s{env};
+    const std::vector<uint32_t> seqs = s.seqs(a.v[1]);
+    const uint32_t cache = s.id(a.v[0]), q = s.id(a.v[2]);
+    const double scale = s.number(a.v[3], "paged cache attend: the scale must be a number");
+    if (!s.ok) return nullptr;
+    return ret_id(env, mni_paged_cache_attend(cache, seqs.data(), seqs.size(), q, scale, get_bool(env, a.v[4]) ? 1 : 0));
 }
 napi_value PagedCacheAddWeights(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    std::vector<uint32_t> seqs;
-    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
-    return ret_rc(env, mni_paged_cache_add_weights(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_u32(env, a.v[2])));
+    Strict s{env};
+    const std::vector<uint32_t> seqs = s.seqs(a.v[1]);
+    const uint32_t cache = s.id(a.v[0]), w = s.id(a.v[2]);
+    if (!s.ok) return nullptr;
+    return ret_rc(env, mni_paged_cache_add_weights(cache, seqs.data(), seqs.size(), w));
 }
 napi_value PagedCacheEvict(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    std::vector<uint32_t> seqs;
-    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
-    return ret_rc(env, mni_paged_cache_evict(get_u32(env, a.v[0]), seqs.data(), seqs.size(), get_i64(env, a.v[2]), get_i64(env, a.v[3])));
+    Strict s{env};
+    const std::vector<uint32_t> seqs = s.seqs(a.v[1]);
+    const uint32_t cache = s.id(a.v[0]);
+    const int64_t budget = s.count(a.v[2]), recent = s.count_or_zero(a.v[3]);
+    if (!s.ok) return nullptr;
+    return ret_rc(env, mni_paged_cache_evict(cache, seqs.data(), seqs.size(), budget, recent));
 }
 napi_value PagedCacheTrack(napi_env env, napi_callback_info info) {
     Args a(env, info);
-    std::vector<uint32_t> seqs;
-    if (!get_list(env, a.v[1], &seqs, WANT_SEQS)) return nullptr;
+    Strict s{env};
+    const std::vector<uint32_t> seqs = s.seqs(a.v[1]);
+    const uint32_t cache = s.id(a.v[0]);
     uint32_t w = 0, p = 0;
-    const int rc = mni_paged_cache_track(get_u32(env, a.v[0]), seqs.data(), seqs.size(), &w, &p);
+    if (!s.ok) return nullptr;
+    const int rc = mni_paged_cache_track(cache, seqs.data(), seqs.size(), &w, &p);
     return ret_ids(env, rc, w, p);
 }
 napi_value PagedCacheRead(napi_env env, napi_callback_info info) {
     Args a(env, info);
+    Strict s{env};
+    const uint32_t cache = s.id(a.v[0]), seq = s.id(a.v[1]);
     uint32_t out[2] = {0, 0};
-    const int rc = mni_paged_cache_read(get_u32(env, a.v[0]), get_u32(env, a.v[1]), out);
+    if (!s.ok) return nullptr;
+    const int rc = mni_paged_cache_read(cache, seq, out);
     return ret_ids(env, rc, out[0], out[1]);
 }
 napi_value PowOp(napi_env env, napi_callback_info info) {  // lib.rs:381-386
