@@ -393,7 +393,8 @@ napi_value QkNormRope(napi_env env, napi_callback_info info) {
     const int64_t offset = s.count_or_zero(a.v[5]), rotary = s.count(a.v[6]);
     const double theta = s.number(a.v[8], "qkNormRope: theta must be a number"), eps = s.number(a.v[9], "qkNormRope: eps must be a number");
     if (!s.ok) return nullptr;
-    return ret_ids(env, mni_qk_norm_rope(in[0], in[1], in[2], in[3], positions, offset, rotary, get_bool(env, a.v[7]) ? 1 : 0, theta, eps, out), out[0], out[1]);
+    const int rc = mni_qk_norm_rope(in[0], in[1], in[2], in[3], positions, offset, rotary, get_bool(env, a.v[7]) ? 1 : 0, theta, eps, out);
+    return ret_ids(env, rc, out[0], out[1]);
 }
 napi_value PagedCacheCreate(napi_env env, napi_callback_info info) {
     Args a(env, info);
