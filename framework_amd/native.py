@@ -224,6 +224,19 @@ def _packed(kind, values):
         raise MniError("id or length out of range: %s" % e)
 
 
+def _uid(v):
+    """An id as ctypes takes it: what does not fit 32 bits is an error, where ctypes would cut it to another id."""
+    if not 0 <= v <= 0xffffffff:
+        raise MniError("id or length out of range: %r" % (v,))
+    return v
+
+
+def _length(v):
+    if not -(1 << 63) <= v < 1 << 63:
+        raise MniError("id or length out of range: %r" % (v,))
+    return v
+
+
 class Rocm:
     """Kernel-level ABI on raw device pointers."""
 
@@ -592,16 +605,16 @@ class Native:
 
     def qkNormRope(self, q, k, gammaQ, gammaK, positions, offset, rotaryDims, interleaved, theta, eps):
         out = (C.c_uint32 * 2)()
-        self._rc(self.lib.mni_qk_norm_rope(q, k, gammaQ, gammaK, BAD_ID if positions is None else positions, offset, rotaryDims,
+        self._rc(self.lib.mni_qk_norm_rope(q, k, gammaQ, gammaK, BAD_ID if positions is None else _uid(positions), _length(offset), _length(rotaryDims),
                                            1 if interleaved else 0, theta, eps, out))
         return [int(out[0]), int(out[1])]
 
     def pagedCacheCreate(self, maxSequences, maxSeqLen, numPages, pageSize, numKvHeads, headDim, quantized, tracked):
-        return self._id(self.lib.mni_paged_cache_create(maxSequences, maxSeqLen, numPages, pageSize, numKvHeads, headDim, 1 if quantized else 0,
+        return self._id(self.lib.mni_paged_cache_create(*map(_length, (maxSequences, maxSeqLen, numPages, pageSize, numKvHeads, headDim)), 1 if quantized else 0,
                                                         1 if tracked else 0))
 
     def pagedCacheFree(self, cacheId):
-        self.lib.mni_paged_cache_free(cacheId)
+        self.lib.mni_paged_cache_free(_uid(cacheId))
 
     def _count(self, v):
         if v < 0:
@@ -609,50 +622,50 @@ class Native:
         return int(v)
 
     def pagedCacheFreePages(self, cacheId):
-        return self._count(self.lib.mni_paged_cache_free_pages(cacheId))
+        return self._count(self.lib.mni_paged_cache_free_pages(_uid(cacheId)))
 
     def pagedCacheAdd(self, cacheId):
-        return self._id(self.lib.mni_paged_cache_add(cacheId))
+        return self._id(self.lib.mni_paged_cache_add(_uid(cacheId)))
 
     def pagedCacheFork(self, cacheId, seq):
-        return self._id(self.lib.mni_paged_cache_fork(cacheId, seq))
+        return self._id(self.lib.mni_paged_cache_fork(_uid(cacheId), _uid(seq)))
 
     def pagedCacheDrop(self, cacheId, seq):
-        self._rc(self.lib.mni_paged_cache_drop(cacheId, seq))
+        self._rc(self.lib.mni_paged_cache_drop(_uid(cacheId), _uid(seq)))
 
     def pagedCacheLen(self, cacheId, seq):
-        return self._count(self.lib.mni_paged_cache_len(cacheId, seq))
+        return self._count(self.lib.mni_paged_cache_len(_uid(cacheId), _uid(seq)))
 
     def pagedCacheSeen(self, cacheId, seq):
-        return self._count(self.lib.mni_paged_cache_seen(cacheId, seq))
+        return self._count(self.lib.mni_paged_cache_seen(_uid(cacheId), _uid(seq)))
 
     def pagedCacheAppend(self, cacheId, seqs, k, v, counts=None):
         if counts is not None and len(counts) != len(seqs):
             raise MniError("paged cache append: %d counts for %d sequences" % (len(counts), len(seqs)))
-        self._rc(self.lib.mni_paged_cache_append(cacheId, _packed("I", seqs), len(seqs), k, v, None if counts is None else _packed("q", counts)))
+        self._rc(self.lib.mni_paged_cache_append(_uid(cacheId), _packed("I", seqs), len(seqs), k, v, None if counts is None else _packed("q", counts)))
 
     def pagedCacheTruncate(self, cacheId, seqs, lens):
         if len(lens) != len(seqs):
             raise MniError("paged cache truncate: %d lengths for %d sequences" % (len(lens), len(seqs)))
-        self._rc(self.lib.mni_paged_cache_truncate(cacheId, _packed("I", seqs), len(seqs), _packed("q", lens)))
+        self._rc(self.lib.mni_paged_cache_truncate(_uid(cacheId), _packed("I", seqs), len(seqs), _packed("q", lens)))
 
     def pagedCacheAttend(self, cacheId, seqs, q, scale, accumulate):
-        return self._id(self.lib.mni_paged_cache_attend(cacheId, _packed("I", seqs), len(seqs), q, scale, 1 if accumulate else 0))
+        return self._id(self.lib.mni_paged_cache_attend(_uid(cacheId), _packed("I", seqs), len(seqs), q, scale, 1 if accumulate else 0))
 
     def pagedCacheAddWeights(self, cacheId, seqs, w):
-        self._rc(self.lib.mni_paged_cache_add_weights(cacheId, _packed("I", seqs), len(seqs), w))
+        self._rc(self.lib.mni_paged_cache_add_weights(_uid(cacheId), _packed("I", seqs), len(seqs), w))
 
     def pagedCacheEvict(self, cacheId, seqs, budget, recent):
-        self._rc(self.lib.mni_paged_cache_evict(cacheId, _packed("I", seqs), len(seqs), budget, recent))
+        self._rc(self.lib.mni_paged_cache_evict(_uid(cacheId), _packed("I", seqs), len(seqs), _length(budget), _length(recent)))
 
     def pagedCacheTrack(self, cacheId, seqs):
         w, p = C.c_uint32(0), C.c_uint32(0)
-        self._rc(self.lib.mni_paged_cache_track(cacheId, _packed("I", seqs), len(seqs), C.byref(w), C.byref(p)))
+        self._rc(self.lib.mni_paged_cache_track(_uid(cacheId), _packed("I", seqs), len(seqs), C.byref(w), C.byref(p)))
         return [w.value, p.value]
 
     def pagedCacheRead(self, cacheId, seq):
         out = (C.c_uint32 * 2)()
-        self._rc(self.lib.mni_paged_cache_read(cacheId, seq, out))
+        self._rc(self.lib.mni_paged_cache_read(_uid(cacheId), _uid(seq), out))
         return [int(out[0]), int(out[1])]
 
     def expOp(self, a):
