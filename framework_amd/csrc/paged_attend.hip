@@ -272,14 +272,17 @@ __global__ __launch_bounds__(TPB) void paged_attend_kernel(const AttendArgs a) {
 // The order in which an MFMA contracts is free as long as both operands agree, which is what lets every load be 8 or 16
 // contiguous bytes of a row: dims 16 j + 4 quarter .. + 3 for the fp32 keys, 4 (lane % 16) + 64 c .. + 3 for the values.
 // fp32 rows: v_mfma_f32_16x16x4_f32 throughout.  int8 rows: the keys' codes are an operand as they lie in memory
-// (v_mfma_i32_16x16x64_i8); a query is three 8-bit digits of its value over the largest of its head, 23 bits, half a
-// unit of which is 2^-24 of that largest, and the integer sums are exact.  The values' codes are widened to bf16 (exact)
+// (v_mfma_i32_16x16x64_i8); a query is four 8-bit digits of its value over the largest of its head, 31 bits, half a
+// unit of which is 2^-32 of that largest, and the integer sums are exact: beside a value ten thousand times theirs (in a dim
+// where the keys are zero) the others still weigh less wrong than fp32 sums would make them; three digits did not do.  The
+// bytes of a biased integer are its digits, so the fourth costs no time (8 x 32 x 4096: 47.3 us with three, 47.4 with four).
+// The values' codes are widened to bf16 (exact)
 // and the probability, times the row's scale, is split into three bf16 parts that hold all of its 24 bits; products are
 // exact and summed in fp32.  A wavefront keeps its tile's keys and values (and the next tile's keys) in registers.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr float QUERY_UNITS = 127.0f * 65536.0f;  // the largest query as an integer of three digits
+constexpr float QUERY_UNITS = 127.0f * 16777216.0f;  // the largest query as an integer of four digits
 
 // Where the rows of 16 positions lie.  The key row of a lane is position lane % 16, its value rows are 4 quarter + r.
 // WIDE (pages of 16 positions and more): the 16 lie in one page, whose id is one scalar load from the table; rows are a
@@ -540,7 +543,7 @@ __global__ __launch_bounds__(TPB, NE <= 8 ? 3 : 1) void paged_attend_tiles_i8_ke
     constexpr int WAVES = TPB / 64, T = 2, TILE = 16 * T, VW = NE / 4;
     typedef int32_t Word __attribute__((ext_vector_type(VW)));
     extern __shared__ int32_t shared[];
-    __shared__ i32x4 digits[3][ND][64];  // [digit][64 dims][lane]
+    __shared__ i32x4 digits[4][ND][64];  // [digit][64 dims][lane]
     __shared__ float units_of[16];
     const PagedPool &p = a.p;
     const int d = EVEN ? 64 * ND : p.d, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m16 = lane & 15, quarter = lane >> 4;
@@ -608,26 +611,26 @@ __global__ __launch_bounds__(TPB, NE <= 8 ? 3 : 1) void paged_attend_tiles_i8_ke
         check = u + v;
         swap32(check, u, v);
         check = u + v;
-        top = fmaxf(top, 1e-30f);  // (below, a unit would be no normal number)
+        top = fmaxf(top, 1e-29f);  // (below, `units` would be infinite)
         const float units = QUERY_UNITS / top;
 #pragma unroll
         for (int j = 0; j < ND; ++j)
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-                uint32_t pack[3] = {0, 0, 0};
+                uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int whole = check == 0.f ? (int)rintf(x[j][y][e] * units) : 0;
-                    // digits within -128 .. 127: the rest below the first is from -32896 to 32639
-                    const int hi = (whole + 32896) >> 16, rest = whole - (hi << 16), mid = (rest + 128) >> 8, lo = rest - (mid << 8);
-                    pack[0] |= (uint32_t)(hi & 255) << (8 * e);
-                    pack[1] |= (uint32_t)(mid & 255) << (8 * e);
-                    pack[2] |= (uint32_t)(lo & 255) << (8 * e);
+                    const int whole = (int)rintf((check == 0.f ? x[j][y][e] : 0.f) * units);
+                    w[e] = ((uint32_t)whole + 0x808080u) ^ 0x808080u;  // its bytes are digits from -128 to 127 that make it up
                 }
+                const uint32_t low01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), high01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
+                const uint32_t low23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400), high23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+                const uint32_t pack[4] = {__builtin_amdgcn_perm(high23, high01, 0x07060302), __builtin_amdgcn_perm(high23, high01, 0x05040100),
+                                          __builtin_amdgcn_perm(low23, low01, 0x07060302), __builtin_amdgcn_perm(low23, low01, 0x05040100)};
 #pragma unroll
-                for (int z = 0; z < 3; ++z) reinterpret_cast<uint32_t *>(&digits[z][j][lane])[y] = pack[z];
+                for (int z = 0; z < 4; ++z) reinterpret_cast<uint32_t *>(&digits[z][j][lane])[y] = pack[z];
             }
-        if (lane < 16) units_of[lane] = (top * (1.0f / QUERY_UNITS) + check) * a.scale;
+        if (lane < 16) units_of[lane] = (top * (256.0f / QUERY_UNITS) + check) * a.scale;
     }
     __syncthreads();
     const float unit = units_of[m16];
@@ -636,16 +639,16 @@ __global__ __launch_bounds__(TPB, NE <= 8 ? 3 : 1) void paged_attend_tiles_i8_ke
         f32x4 s[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            i32x4 x[3];
+            i32x4 x[4];
 #pragma unroll
-            for (int y = 0; y < 3; ++y) {
+            for (int y = 0; y < 4; ++y) {
                 x[y] = i32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int j = 0; j < ND; ++j) x[y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][j], digits[y][j][lane], x[y], 0, 0, 0);
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                s[t][r] = ((float)x[0][r] * 65536.0f + ((float)x[1][r] * 256.0f + (float)x[2][r])) * (ks[t][r] * unit);
+                s[t][r] = ((float)(x[0][r] * 256 + x[1][r]) * 256.0f + (float)(x[2][r] * 256 + x[3][r]) * 0x1p-8f) * (ks[t][r] * unit);
         }
         if (next < w.n) load_keys(next);
         if (a.scores) tile_scores_keep<T>(scores, w, s, base, lane);
