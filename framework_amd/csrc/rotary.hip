@@ -26,7 +26,7 @@ struct RopeArgs {
     uint32_t first;  // forward: workgroups of the launches before
     int d, rot, interleaved;
     float eps, inv_d;
-    double turns[ROPE_MAX_DIM / 2];  // theta^(-2i / rot) / (2 pi): turns per position of pair i
+    double quarters[ROPE_MAX_DIM / 2];  // theta^(-2i / rot) / (pi / 2): quarter turns per position of pair i
 };
 
 // Eight values of a row per lane, as two pieces of four.  Rotated dims: with split halves lane l holds 4l .. 4l + 3 of
@@ -44,22 +44,35 @@ __device__ __forceinline__ RopePlace rope_place(const RopeArgs &a, int l) {
     else { p.lo = a.rot + 8 * (l - a.rot / 8); p.hi = p.lo + 4; }
     return p;
 }
+// cos and sin of at * f quarter turns.  In 64 bits, less whole quarter turns (1.5 * 2^52 added leaves the nearest whole number in
+// the sum's last bits, whose last two are the quadrant); the rest, half a quarter turn at most, is rounded to 32 bits, which costs
+// 0.4 * 2^-24, and goes through the Taylor polynomials of sin(pi r / 2) to r^9 and cos(pi r / 2) to r^10 (the next terms are
+// below 2^-28).  Off by 1.4 * 2^-24 at most, and by three half steps of the result where that is small; the fraction of a whole
+// turn rounded to 32 bits before sincospif was off by 1.8, by all bits next to a zero, and took 54.0 us where this takes 53.5 (8 x
+// 1024 x 24 rows of 64, both ways).  Far positions add the frequency's rounding, 1.5 * 2^-53 of the angle.
+__device__ __forceinline__ void rope_turn(double at, double f, float &c, float &s) {
+    const double shift = 6755399441055744.0, moved = fma(at, f, shift);
+    const uint32_t quadrant = (uint32_t)__double2loint(moved);
+    const float r = (float)fma(at, f, shift - moved), z = r * r;
+    const float tail = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 1.6044118e-4f, -4.6817541e-3f), 7.9692626e-2f), -6.4596410e-1f), -4.3711388e-8f);
+    const float sine = fmaf(r, 1.57079637f, r * tail);  // (pi / 2 in two parts)
+    const float cosine = fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -2.5202042e-5f, 9.1926027e-4f), -2.0863481e-2f), 2.5366951e-1f), -1.2337006f), 1.0f);
+    const bool odd = quadrant & 1;
+    s = __uint_as_float(__float_as_uint(odd ? cosine : sine) ^ ((quadrant & 2) << 30));
+    c = __uint_as_float(__float_as_uint(odd ? sine : cosine) ^ (((quadrant + 1) & 2) << 30));
+}
 // cos and sin of the four pairs of a lane (pairs lo .. lo + 3; interleaved: lo / 2, lo / 2 + 1, hi / 2, hi / 2 + 1).
-// position * turns in 64 bits, less whole turns: the fraction keeps 24 good bits for any 32-bit position.
 __device__ __forceinline__ void rope_angles(const RopeArgs &a, const double (&f)[4], uint32_t token, float (&c)[4], float (&s)[4]) {
     const uint32_t b = token / a.seq, t = token - b * a.seq;
     const double at = (double)((a.positions ? (int64_t)a.positions[b * a.position_stride + t] : (int64_t)t) + a.offset);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const double turn = at * f[j];
-        sincospif((float)(2.0 * (turn - rint(turn))), &s[j], &c[j]);
-    }
+    for (int j = 0; j < 4; ++j) rope_turn(at, f[j], c[j], s[j]);
 }
-__device__ __forceinline__ void rope_turns(const RopeArgs &a, const RopePlace &p, double (&f)[4]) {
+__device__ __forceinline__ void rope_quarters(const RopeArgs &a, const RopePlace &p, double (&f)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int pair = a.interleaved ? (j < 2 ? p.lo / 2 + j : p.hi / 2 + j - 2) : p.lo + j;
-        f[j] = p.turning ? a.turns[pair] : 0.0;
+        f[j] = p.turning ? a.quarters[pair] : 0.0;
     }
 }
 // (v0 .. v7) turned by +angle (SIGN 1) or -angle (SIGN -1)
@@ -107,7 +120,7 @@ __global__ __launch_bounds__(ROPE_TPB) void rope_forward_kernel(const RopeArgs a
     const RopePlace p = rope_place(a, threadIdx.x % LPR);
     const int heads = (int)(a.q.heads + a.k.heads);
     double f[4];
-    rope_turns(a, p, f);
+    rope_quarters(a, p, f);
     float v[HPG][8];
 #pragma unroll
     for (int j = 0; j < HPG; ++j) {
@@ -145,7 +158,7 @@ __global__ __launch_bounds__(ROPE_TPB) void rope_backward_kernel(const RopeArgs 
     const int group = threadIdx.x / LPR, l = threadIdx.x % LPR;
     const RopePlace p = rope_place(a, l);
     double f[4];
-    rope_turns(a, p, f);
+    rope_quarters(a, p, f);
     float g[8], acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
@@ -216,8 +229,7 @@ __device__ __forceinline__ void rope_pair(const RopeArgs &a, int i, int &lo, int
 }
 __device__ __forceinline__ void rope_sincos(const RopeArgs &a, uint32_t token, int i, float &c, float &s) {
     const uint32_t b = token / a.seq, t = token - b * a.seq;
-    const double turn = (double)((a.positions ? (int64_t)a.positions[b * a.position_stride + t] : (int64_t)t) + a.offset) * a.turns[i];
-    sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
+    rope_turn((double)((a.positions ? (int64_t)a.positions[b * a.position_stride + t] : (int64_t)t) + a.offset), a.quarters[i], c, s);
 }
 __global__ __launch_bounds__(ROPE_TPB) void rope_forward_any_kernel(const RopeArgs a) {
     const int heads = (int)(a.q.heads + a.k.heads), lane = threadIdx.x & 63;
@@ -339,14 +351,14 @@ int rope_args(const mni_rope_desc &d, bool backward, RopeArgs *a) {
     a->eps = (float)d.eps;
     a->inv_d = 1.0f / (float)d.head_dim;
     // The last plan's frequencies are kept (a model has one): 64 powers cost as long as a launch.
-    static double turns[ROPE_MAX_DIM / 2], of_theta = 0.0;
+    static double quarters[ROPE_MAX_DIM / 2], of_theta = 0.0;
     static int of_rot = -1;
     if (of_theta != d.theta || of_rot != a->rot) {
-        for (int i = 0; i < ROPE_MAX_DIM / 2; ++i) turns[i] = i < a->rot / 2 ? pow(d.theta, -2.0 * i / a->rot) / (2.0 * M_PI) : 0.0;
+        for (int i = 0; i < ROPE_MAX_DIM / 2; ++i) quarters[i] = i < a->rot / 2 ? pow(d.theta, -2.0 * i / a->rot) / M_PI_2 : 0.0;
         of_theta = d.theta;
         of_rot = a->rot;
     }
-    memcpy(a->turns, turns, sizeof turns);
+    memcpy(a->quarters, quarters, sizeof quarters);
     return MNI_OK;
 }
 // `blocks` workgroups, in as many launches as grids are needed for them.

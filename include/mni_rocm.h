@@ -261,7 +261,8 @@ int mni_rocm_fill(float *dst, float value, int64_t n);
  *   y[lo] = z[lo] cos a - z[hi] sin a,  y[hi] = z[hi] cos a + z[lo] sin a,  the values from rotary_dims on unrotated,
  * with a = (position + offset) * theta^(-2 i / rotary_dims) for pair i = 0 .. rotary_dims / 2 - 1, which is (i, i +
  * rotary_dims / 2), or (2i, 2i + 1) when `interleaved`.  Angles are formed in 64 bits and reduced to a fraction of a
- * turn before the 32-bit sine and cosine, so a far position is as exact as a near one.
+ * turn before the 32-bit sine and cosine, which are off by 1.4 half steps of 1 at most; a far position is as exact as a near
+ * one up to about 2^27, at 2^31 the 64-bit angle itself may be off by another six.
  * `heads` rows per token, x[b, h, s, :] = x + b * batch_stride + h * head_stride + s * token_stride (elements, the
  * last extent contiguous: a projection's output, or its part of a fused one, is read where it lies); outputs
  * contiguous [batch, heads, seq, head_dim].  heads == 0 leaves that operand out.
