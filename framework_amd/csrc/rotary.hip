@@ -324,6 +324,9 @@ int rope_args(const mni_rope_desc &d, bool backward, RopeArgs *a) {
         return set_error(MNI_ERR_INVALID, "%s: rotary_dims %lld must be even and at most head_dim %lld", what, (long long)d.rotary_dims, (long long)d.head_dim);
     if (!(d.theta > 0.0) || !isfinite(d.theta)) return set_error(MNI_ERR_INVALID, "%s: theta must be positive", what);
     if (!(d.eps >= 0.0) || !isfinite(d.eps)) return set_error(MNI_ERR_INVALID, "%s: eps must not be negative", what);
+    const int64_t far = (int64_t)1 << 32;
+    if (d.offset < -far || d.offset > far)  // (the 64-bit angle loses its fraction on the way, and beside INT64_MAX the sum its sign)
+        return set_error(MNI_ERR_INVALID, "%s: offset %lld beyond 2^32", what, (long long)d.offset);
     const int64_t most = (int64_t)1 << 31;
     if (d.seq > most || d.batch > most || d.q.heads > (1 << 20) || d.k.heads > (1 << 20) || (d.seq && d.batch > most / d.seq))
         return set_error(MNI_ERR_INVALID, "%s: more than 2^31 tokens or 2^20 heads", what);
@@ -350,7 +353,7 @@ int rope_args(const mni_rope_desc &d, bool backward, RopeArgs *a) {
     a->first = 0;
     a->eps = (float)d.eps;
     a->inv_d = 1.0f / (float)d.head_dim;
-    // The last plan's frequencies are kept (a model has one): 64 powers cost as long as a launch.
+    // The last plan's frequencies are kept: 64 powers take as long as a launch (calls that alternate between two plans pay that).
     static double quarters[ROPE_MAX_DIM / 2], of_theta = 0.0;
     static int of_rot = -1;
     if (of_theta != d.theta || of_rot != a->rot) {
