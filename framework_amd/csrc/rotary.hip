@@ -1,8 +1,8 @@
 // Norm of queries and keys for each head with the rotation of their positions in the same pass, and its backward
 // (mni_rocm_qk_norm_rope).  Bound by bandwidth where there are many rows: 8 bytes an element forward (one read, one
 // write), 12 backward, and both run at the rate of a large copy (5.6 TB/s; less than the whole traffic need reach HBM):
-// forward 5.7 TB/s on 2047 x 40 rows of 128 values (84 MB, 14.6 us), 6.2 on 8192 x 24 of 64 (101 MB, 16.2 us), backward
-// 5.8 there (151 MB, 25.8 us).  A decoding step's 8 x 24 rows are one launch, 3.7 us.  All sums are fp32, the angles 64-bit.
+// forward 5.8 TB/s on 2047 x 40 rows of 128 values (84 MB, 14.5 us), 6.3 on 8192 x 24 of 64 (101 MB, 16.0 us), backward
+// 5.9 there (151 MB, 25.4 us).  A decoding step's 8 x 24 rows are one launch, 3.6 us.  All sums are fp32, the angles 64-bit.
 #include <math.h>
 #include <string.h>
 
