@@ -323,6 +323,8 @@ int rope_args(const mni_rope_desc &d, bool backward, RopeArgs *a) {
     if (d.rotary_dims < 0 || d.rotary_dims > d.head_dim || d.rotary_dims % 2)
         return set_error(MNI_ERR_INVALID, "%s: rotary_dims %lld must be even and at most head_dim %lld", what, (long long)d.rotary_dims, (long long)d.head_dim);
     if (!(d.theta > 0.0) || !isfinite(d.theta)) return set_error(MNI_ERR_INVALID, "%s: theta must be positive", what);
+    if (d.theta < 0x1p-16)  // (a position below 2^33 then stays below 2^49 quarter turns, which rope_turn takes apart; from 1 on, below 2^33)
+        return set_error(MNI_ERR_INVALID, "%s: theta %g below 2^-16", what, d.theta);
     if (!(d.eps >= 0.0) || !isfinite(d.eps)) return set_error(MNI_ERR_INVALID, "%s: eps must not be negative", what);
     const int64_t far = (int64_t)1 << 32;
     if (d.offset < -far || d.offset > far)  // (the 64-bit angle loses its fraction on the way, and beside INT64_MAX the sum its sign)

@@ -268,7 +268,7 @@ int mni_rocm_fill(float *dst, float value, int64_t n);
  * contiguous [batch, heads, seq, head_dim].  heads == 0 leaves that operand out.
  * positions: seq int32 values, of sequence b at positions + b * position_stride (0: shared by all); NULL: 0 .. seq - 1.
  * Errors: head_dim not in 1 .. 256, rotary_dims odd, negative or beyond head_dim, theta or eps not positive
- * (eps may be 0), offset beyond 2^32 either way. */
+ * (eps may be 0), theta below 2^-16, offset beyond 2^32 either way. */
 typedef struct {
     const float *x;
     int64_t heads, batch_stride, head_stride, token_stride;
