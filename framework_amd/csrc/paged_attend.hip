@@ -274,8 +274,8 @@ __global__ __launch_bounds__(TPB) void paged_attend_kernel(const AttendArgs a) {
 // fp32 rows: v_mfma_f32_16x16x4_f32 throughout.  int8 rows: the keys' codes are an operand as they lie in memory
 // (v_mfma_i32_16x16x64_i8); a query is four 8-bit digits of its value over the largest of its head, 31 bits, half a
 // unit of which is 2^-32 of that largest, and the integer sums are exact: beside a value ten thousand times theirs (in a dim
-// where the keys are zero) the others still weigh less wrong than fp32 sums would make them; three digits did not do.  The
-// bytes of a biased integer are its digits, so the fourth costs no time (8 x 32 x 4096: 47.3 us with three, 47.4 with four).
+// where the keys are zero) the others' scores stay within the bound of fp32 sums, which three digits left.  The bytes of a
+// biased integer are its digits, so the fourth costs no time (8 x 32 x 4096: 47.3 us with three, 47.4 with four).
 // The values' codes are widened to bf16 (exact)
 // and the probability, times the row's scale, is split into three bf16 parts that hold all of its 24 bits; products are
 // exact and summed in fp32.  A wavefront keeps its tile's keys and values (and the next tile's keys) in registers.

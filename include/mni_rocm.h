@@ -484,8 +484,9 @@ int mni_qk_norm_rope(uint32_t q, uint32_t k, uint32_t gamma_q, uint32_t gamma_k,
  * read: keys and values of one sequence in the order held, [kv_heads, len, head_dim] (int8 rows as the values they
  *   stand for).
  * Like mni_kv_cache_*, these are for answering: nothing is recorded on the tape.  Scores, maxima, sums and outputs are
- * fp32 (against int8 rows a query's value may be held to 2^-32 of the largest value of its head); an int8 row is stored as round(x (1 / s)) with s = max |x| (1 / 127), at least 1e-8, each step in fp32.  An int8
- * row that holds an infinity or a NaN is NaN throughout, as read and as attended to. */
+ * fp32 (against int8 rows a query's value may be held to 2^-32 of the largest value of its head); an int8 row is stored
+ * as round(x (1 / s)) with s = max |x| (1 / 127), at least 1e-8, each step in fp32.  An int8 row that holds an infinity or
+ * a NaN is NaN throughout, as read and as attended to. */
 uint32_t mni_paged_cache_create(int64_t max_sequences, int64_t max_seq_len, int64_t num_pages, int64_t page_size, int64_t kv_heads,
                                 int64_t head_dim, int quantized, int tracked);
 void mni_paged_cache_free(uint32_t cache_id);
